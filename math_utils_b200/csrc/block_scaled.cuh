@@ -1,0 +1,91 @@
+// Numbers in 8 and 4 bits with a power-of-two scale for every 32 along a row.
+//
+// A group of 32 entries v is kept as codes c and one exponent byte b (0..254): v = c * 2^(b - 127).  Rows take the
+// codes e4m3 (a sign, four exponent and three mantissa bits, up to 448), weights e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a
+// sign).  The exponent of a row's group is the smallest at which its largest entry is no larger than 448.
+//
+// Exponent bytes lie as the tensor cores read them: tiles of 128 rows by 128 columns, 512 bytes each, the tiles of a row
+// of tiles one after another; within a tile row r has its four bytes at (r % 32) * 16 + (r / 32) * 4.
+#pragma once
+#include "common.cuh"
+
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+
+namespace mu {
+
+constexpr int BS_GROUP = 32;               // entries that share a scale
+constexpr int BS_TILE = 128;               // rows and columns of a tile of scales
+constexpr int BS_TILE_BYTES = 512;
+
+// Where the exponent byte of (row, group) lies; kb: tiles along a row.
+__host__ __device__ __forceinline__ long long scale_at(long long row, int group, int kb) {
+    return ((row / BS_TILE) * kb + group / 4) * BS_TILE_BYTES + (row % 32) * 16 + (row % BS_TILE) / 32 * 4 + group % 4;
+}
+
+// The exponent byte for a group whose largest magnitude is `top` (finite): the smallest b with top <= 448 * 2^(b - 127).
+// 448 = 1.75 * 2^8, so b is the exponent field of top less 8, and one more where top's mantissa is above 1.75.
+__device__ __forceinline__ int exponent_e4m3(float top) {
+    const unsigned int bits = __float_as_uint(top);
+    const int b = (int)(bits >> 23) - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return b > 0 ? b : 0;
+}
+// The same for e2m1, whose largest value is 6 = 1.5 * 2^2.
+__device__ __forceinline__ int exponent_e2m1(float top) {
+    const unsigned int bits = __float_as_uint(top);
+    const int b = (int)(bits >> 23) - 2 + ((bits & 0x7FFFFFu) > 0x400000u ? 1 : 0);
+    return b > 0 ? (b < 254 ? b : 254) : 0;
+}
+// 2^(127 - b), by which a group's entries are multiplied on the way to their codes (exact: a power of two).
+__device__ __forceinline__ float inverse_scale(int b) { return __uint_as_float((unsigned int)(254 - b) << 23); }
+__device__ __forceinline__ float scale_value(int b) { return b > 0 ? __uint_as_float((unsigned int)b << 23) : __uint_as_float(0x00400000u); }
+
+__device__ __forceinline__ bool is_finite_magnitude(float top) { return __float_as_uint(top) < 0x7F800000u; }
+// The larger magnitude; NaN where either is NaN (so that a group holding one is seen).
+__device__ __forceinline__ float larger_magnitude(float a, float b) {
+    a = fabsf(a);
+    b = fabsf(b);
+    return (a > b || a != a) ? a : b;
+}
+
+__device__ __forceinline__ unsigned int e4m3_pair(float lo, float hi) {
+    return (unsigned int)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float2 of_e4m3_pair(unsigned int pair) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)pair, __NV_E4M3);
+    return __half22float2(__half2(h));
+}
+
+constexpr unsigned int E4M3_NAN4 = 0x7F7F7F7Fu;
+
+// Eight entries of a group of exponent byte b, as codes.
+__device__ __forceinline__ uint2 e4m3_of_eight(const float (&v)[8], int b) {
+    const float f = inverse_scale(b);
+    uint2 c;
+    c.x = e4m3_pair(v[0] * f, v[1] * f) | e4m3_pair(v[2] * f, v[3] * f) << 16;
+    c.y = e4m3_pair(v[4] * f, v[5] * f) | e4m3_pair(v[6] * f, v[7] * f) << 16;
+    return c;
+}
+
+// Eight bfloat16 entries of a group as TWO codes each: hi = e4m3(v / 2^e), lo = e4m3((v - hi 2^e) / 2^(e - 4)), so that
+// v = hi 2^e + lo 2^(e - 4).  A bfloat16 has 8 significant bits, hi takes the upper 4 and leaves a remainder of at most
+// 2^-4 of v that is a multiple of 2^-7 of v's leading bit: 4 bits, which lo holds exactly.  (Entries below 2^-14 of the
+// group's largest lose what lies below 2^-22 of that largest one.)  The exponent byte of lo is b - 4; where b < 4 (a
+// group below 2^-115) its scale stays at 2^-127 and lo is made for that scale.
+__device__ __forceinline__ int low_exponent(int b) { return b > 4 ? b - 4 : 0; }
+__device__ __forceinline__ void e4m3_pieces_of_eight(const float (&v)[8], int b, uint2& hi, uint2& lo) {
+    const float s = scale_value(b), fl = inverse_scale(low_exponent(b));
+    hi = e4m3_of_eight(v, b);
+    float r[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 h = of_e4m3_pair(((i < 2 ? hi.x : hi.y) >> (16 * (i & 1))) & 0xFFFFu);
+        r[2 * i] = (v[2 * i] - h.x * s) * fl;
+        r[2 * i + 1] = (v[2 * i + 1] - h.y * s) * fl;
+    }
+    lo.x = e4m3_pair(r[0], r[1]) | e4m3_pair(r[2], r[3]) << 16;
+    lo.y = e4m3_pair(r[4], r[5]) | e4m3_pair(r[6], r[7]) << 16;
+}
+
+}  // namespace mu

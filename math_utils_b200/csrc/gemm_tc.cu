@@ -19,10 +19,6 @@ int launch_gemm_pair(int bn, const void* A, const void* W, const float* bias, co
                      long long lda, long long ldw, long long ldc, long long ldr, int act, int out_bf16, int* status,
                      cudaStream_t s);
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 static EncodeTiledFn encode_tiled() {
     static EncodeTiledFn fn = nullptr;
     static std::once_flag once;
@@ -35,6 +31,7 @@ static EncodeTiledFn encode_tiled() {
     });
     return fn;
 }
+EncodeTiledFn encode_tiled_fn() { return encode_tiled(); }
 
 // Descriptors are pure functions of (address, shape, stride, box): the last few hundred are kept, since a
 // model asks for the same ones step after step (weights always, activations whenever the allocator hands

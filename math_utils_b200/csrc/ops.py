@@ -11,7 +11,7 @@ import ctypes
 import functools
 import os
 import threading
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -188,6 +188,14 @@ _SIGNATURES = {
     "mu_rms_norm_pair": [_c_p, _c_ll, _c_p, _c_p, _c_f, _c_p, _c_ll, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_p],
     "mu_softcap": [_c_p, _c_ll, _c_int, _c_int, _c_f, _c_p],
     "mu_moe_tile_rows": [],
+    "mu_verify_scratch": [_c_int] * 3,
+    "mu_verify_drafts": [_c_p, _c_ll, _c_ll, _c_p, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_p, _c_p, ctypes.c_double, _c_int,
+                         _c_int, _c_p, _c_p, _c_p, _c_p],
+    "mu_quantize_q4": [_c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p, _c_p],
+    "mu_quantize_q8": [_c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p, _c_p],
+    "mu_residual_add_norm_q8": [_c_p, _c_ll, _c_p, _c_ll, _c_f, _c_p, _c_ll, _c_f, _c_p, _c_p, _c_f, _c_int, _c_int, _c_int,
+                                _c_p, _c_p, _c_p],
+    "mu_q4_few_rows": [_c_p] * 8 + [_c_p, _c_int, _c_int, _c_int, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_p, _c_p],
     "mu_sample": [_c_p, _c_ll, _c_int, _c_int, _c_f, _c_int, _c_ull, _c_p, _c_p, _c_p, _c_p, _c_p, _c_int,
                   _c_p, _c_p, _c_p],
 }
@@ -1707,6 +1715,175 @@ def gemm_skinny(a: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] =
     return out
 
 
+# ---------------------------------------------------------------- 4-bit weights and 8-bit rows
+class Q4Weight(NamedTuple):
+    """A weight matrix [n, k] in 4 bits with a power-of-two scale for every 32 entries along k.
+
+    ``codes`` (uint8 [n, kp / 2], contiguous, 32-byte aligned; kp: k rounded up to 128): the code of an even column in the
+    low half of its byte; a code is a sign bit above one of 0, 0.5, 1, 1.5, 2, 3, 4, 6; columns from k on are zeros.
+    ``scales`` (float8_e8m0fnu [ceil(n / 128), kp / 128, 32, 4, 4], contiguous): the tile of 128 rows and 128 columns that
+    the tensor cores read at a time; row r of a tile at [r % 32, r // 32], its four groups of 32 columns last."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+class Q8Rows(NamedTuple):
+    """Rows [m, k] in 8 bits with a power-of-two scale for every 32 entries: ``codes`` float8_e4m3fn [m, kp], ``scales``
+    laid out as ``Q4Weight``'s (rows past m have scales that nothing uses, but columns from k on have codes of zero)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def _padded(k: int) -> int:
+    return -(-k // 128) * 128
+
+
+def _on_current_device(*tensors) -> None:
+    """These kernels are launched on the current device's stream: tensors of another device are refused."""
+    _need_cuda(*tensors)
+    current = _current_device() if _current_device is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != current:
+            raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{current}")
+
+
+def _scales_for(rows: int, kp: int, device) -> torch.Tensor:
+    return torch.empty((-(-rows // 128), kp // 128, 32, 4, 4), dtype=torch.float8_e8m0fnu, device=device)
+
+
+def _check_scaled(codes: torch.Tensor, scales: torch.Tensor, kp: int, what: str) -> None:
+    if (scales.dtype != torch.float8_e8m0fnu or scales.numel() * 32 != -(-codes.shape[0] // 128) * 128 * kp
+            or not scales.is_contiguous() or not codes.is_contiguous()):
+        raise KernelError(f"{what}: contiguous codes {tuple(codes.shape)} go with contiguous float8_e8m0fnu scales "
+                          f"[{-(-codes.shape[0] // 128)}, {kp // 128}, 32, 4, 4], got {scales.dtype} {tuple(scales.shape)}")
+
+
+def quantize_q4(w: torch.Tensor) -> Q4Weight:
+    """A matrix [n, k] (bfloat16 or float32, unit stride along k) in 4 bits.  A group's scale is the smallest power of two
+    at which its largest entry is no larger than 6, or the one below where that leaves the smaller sum of squared
+    errors (the largest entries are then cut off at 6); entries go to the nearest code, halves to the even one.  A group
+    that holds an infinity or NaN becomes NaN."""
+    if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1 or w.stride(1) != 1:
+        raise KernelError("quantize_q4 takes a matrix [n, k] with unit stride along k")
+    is_bf16 = _is_bf16(w)
+    _on_current_device(w)
+    n, k = w.shape
+    kp = _padded(k)
+    codes = torch.empty((n, kp // 2), dtype=torch.uint8, device=w.device)
+    scales = _scales_for(n, kp, w.device)
+    _check(library().mu_quantize_q4(_ptr(w), w.stride(0) if n > 1 else k, is_bf16, n, k, kp, _ptr(codes), _ptr(scales), _stream()),
+           ("quantize_q4({}x{})", n, k))
+    return Q4Weight(codes, scales)
+
+
+def quantize_q8(x: torch.Tensor) -> Q8Rows:
+    """Rows [m, k] (bfloat16 or float32, unit stride along k) in 8 bits: a group's scale is the smallest power of two at
+    which its largest entry is no larger than 448, and entries go to the nearest e4m3, halves to the even one.  A
+    group that holds an infinity or NaN becomes NaN."""
+    if x.dim() != 2 or x.shape[1] < 1 or x.stride(1) != 1:
+        raise KernelError("quantize_q8 takes rows [m, k] with unit stride along k")
+    is_bf16 = _is_bf16(x)
+    _on_current_device(x)
+    m, k = x.shape
+    kp = _padded(k)
+    codes = torch.empty((m, kp), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = _scales_for(m, kp, x.device)
+    _check(library().mu_quantize_q8(_ptr(x), x.stride(0), is_bf16, m, k, kp, 1, _ptr(codes), _ptr(scales), _stream()),
+           ("quantize_q8({}x{})", m, k))
+    return Q8Rows(codes, scales)
+
+
+def residual_add_norm_q8(x: torch.Tensor, y: Optional[torch.Tensor], mult: float, weight: torch.Tensor, eps: float,
+                         y2: Optional[torch.Tensor] = None, mult2: float = 0.0,
+                         scale: Optional[torch.Tensor] = None) -> Q8Rows:
+    """``residual_add_norm`` whose normed rows come in 8 bits: x += (mult * y + mult2 * y2) * scale on the float32
+    stream, in place, then x / rms(x) * weight as ``quantize_q8`` would make it from the unrounded values."""
+    if x.dtype != torch.float32 or x.dim() != 2 or x.stride(1) != 1 or x.shape[1] < 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+        raise KernelError("residual_add_norm_q8: the stream is float32 [rows, n] with unit inner stride and rows apart")
+    for t in (y, y2):
+        if t is not None and (t.dtype != torch.float32 or t.shape != x.shape or t.stride(1) != 1):
+            raise KernelError("residual_add_norm_q8: the sublayer's output is float32 and shaped like the stream")
+    m, k = x.shape
+    if (y2 is not None or scale is not None) and y is None or scale is not None and (
+            scale.dtype != torch.float32 or scale.numel() != k or not scale.is_contiguous()):
+        raise KernelError("residual_add_norm_q8: a second branch or a scale (one contiguous float32 per entry) goes with a first branch")
+    if weight.dtype != torch.float32 or weight.numel() != k or not weight.is_contiguous():
+        raise KernelError("residual_add_norm_q8: a contiguous float32 weight of n values")
+    _on_current_device(x, y, weight, y2, scale)
+    kp = _padded(k)
+    codes = torch.empty((m, kp), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = _scales_for(m, kp, x.device)
+    _check(library().mu_residual_add_norm_q8(
+        x.data_ptr(), x.stride(0), _ptr(y), y.stride(0) if y is not None else 0, mult, _ptr(y2),
+        y2.stride(0) if y2 is not None else 0, mult2, _ptr(scale), weight.data_ptr(), eps, m, k, kp, codes.data_ptr(),
+        scales.data_ptr(), _stream()), ("residual_add_norm_q8(n={})", k))
+    return Q8Rows(codes, scales)
+
+
+def linear_q4(x, weight: Q4Weight, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
+              residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+              out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """act(x @ W^T + bias) + residual with W in 4 bits.  ``x``: bfloat16 [m, k] with unit stride along k (taken as they
+    are: cut into two 8-bit pieces that together hold them), ``Q8Rows``, or a ``NormedInput``.  Sums are float32;
+    ``out`` bfloat16 (the default) or float32; ``bias`` float32 [n], ``residual`` float32 [m, n], which may be ``out``.
+    A row that holds an infinity or NaN gives NaN."""
+    if isinstance(x, NormedInput):
+        x = x.materialize()
+    codes, w_scales = weight
+    if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[0] < 1 or codes.shape[1] % 64 or codes.shape[1] == 0:
+        raise KernelError(f"linear_q4: the weight's codes are uint8 [n, kp / 2] with kp a multiple of 128, got {codes.dtype} {tuple(codes.shape)}")
+    n, kp = codes.shape[0], codes.shape[1] * 2
+    _check_scaled(codes, w_scales, kp, "linear_q4, weight")
+    rows = isinstance(x, Q8Rows)
+    if rows:
+        x_codes, x_scales = x
+        if x_codes.dtype != torch.float8_e4m3fn or x_codes.dim() != 2 or x_codes.shape[1] != kp:
+            raise KernelError(f"linear_q4: rows are float8_e4m3fn [m, {kp}], got {x_codes.dtype} {tuple(x_codes.shape)}")
+        _check_scaled(x_codes, x_scales, kp, "linear_q4, rows")
+        m, k = x_codes.shape[0], kp
+    else:
+        if x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1 or not 0 <= kp - x.shape[1] < 128:
+            raise KernelError(f"linear_q4: rows are bfloat16 [m, k] with unit stride along k and k rounded up to 128 equal to "
+                              f"{kp}, or Q8Rows; got {x.dtype} {tuple(x.shape)}")
+        x_codes = x
+        m, k = x.shape
+    if act not in ACT_CODES:
+        raise KernelError(f"linear_q4: the activation is one of {', '.join(str(a) for a in ACT_CODES)}, got {act}")
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype or torch.bfloat16, device=codes.device)
+    elif out.shape != (m, n) or out.stride(1) != 1 or (out_dtype is not None and out.dtype != out_dtype):
+        raise KernelError("gemm output has the wrong shape, stride or dtype")
+    out_bf16 = _is_bf16(out)
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n or not bias.is_contiguous()):
+        raise KernelError("gemm bias must be contiguous float32 of length n")
+    if residual is not None and (residual.dtype != torch.float32 or residual.shape != out.shape or residual.stride(1) != 1):
+        raise KernelError("gemm residual must be float32 [m, n]")
+    _on_current_device(x_codes, codes, w_scales, bias, residual, out, x_scales if rows else None)
+    if m == 0:
+        return out
+    lib, stream = library(), _stream()
+    if rows:
+        at = (x_codes.data_ptr(), x_scales.data_ptr(), None, None)
+        step, tile = kp, kp * 4
+    else:
+        # both pieces' codes, then both pieces' exponents (whole tiles of 128 rows)
+        tiles = -(-m // 128) * (kp * 4)
+        room = torch.empty((2 * m * kp + 2 * tiles,), dtype=torch.uint8, device=codes.device)
+        first = room.data_ptr()
+        _check(lib.mu_quantize_q8(x.data_ptr(), x.stride(0), 1, m, k, kp, 2, first, first + 2 * m * kp, stream), ("quantize_q8({}x{})", m, k))
+        at = (first, first + 2 * m * kp, first + m * kp, first + 2 * m * kp + tiles)
+        step, tile = kp, kp * 4
+    ldr = residual.stride(0) if residual is not None else 0
+    for r0 in range(0, m, 128):
+        here = [None if p is None else p + (r0 * step if i % 2 == 0 else r0 // 128 * tile) for i, p in enumerate(at)]
+        _check(lib.mu_q4_few_rows(
+            *here, codes.data_ptr(), w_scales.data_ptr(), _ptr(bias),
+            None if residual is None else residual.data_ptr() + r0 * ldr * 4, out.data_ptr() + r0 * out.stride(0) * out.element_size(),
+            min(m - r0, 128), n, kp, out.stride(0), ldr, ACT_CODES[act], out_bf16, 0, status_word(codes.device).data_ptr(), stream),
+            ("linear_q4({}x{}x{})", m, n, kp))
+    return out
+
+
 # ------------------------------------------------------------------- attention
 def kv_append(k: torch.Tensor, v: torch.Tensor, tok_pos, tok_seq, block_table: torch.Tensor,
               page_tokens: int, n_kv_heads: int, head_dim: int, kv_pages: torch.Tensor,
@@ -1808,6 +1985,55 @@ def sample(logits: torch.Tensor, temperature: float, top_k: int, seed: int,
                                int(feed[2]) if feed else 0, *_status_args(status_to, logits.device), _stream()),
            "sample")
     return out
+
+
+def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], drafts: torch.Tensor, draws: torch.Tensor,
+                  temperature: float, top_k: int):
+    """Which drafted tokens the target takes: (tokens int32 [batch, drafts + 1], kept int32 [batch]).
+
+    ``logits`` float32 [batch, drafts + 1, vocab]: the target's, row i of a sequence for the place of its draft i and the
+    last row for the place behind them; ``draft_logits`` float32 [batch, drafts, vocab]: what the drafts were sampled from
+    (None where greedy); unit inner stride both.  ``drafts`` int32 [batch, drafts]; a draft of -1 ends a sequence's
+    drafts.  ``draws`` float64 [batch, drafts + 1] in [0, 1).  ``temperature`` and ``top_k`` as ``sample`` has them (0 or
+    less: greedy; 0 or less: all; 1: greedy).
+
+    With p and q the softmax of a target and a draft row over its ``top_k`` largest logits, draft i is taken while
+    draws[i] * q(draft i) < p(draft i).  The token behind the taken ones comes from max(p - q, 0) where a draft was not
+    taken and from p where none is left: the first index at which the running sum passes draws[drafts] of the whole.
+    ``tokens``: the drafts taken, that token, then -1; ``kept`` how many drafts were taken.  Greedy: a draft is taken
+    while it is its row's first maximum, which is also the token that follows."""
+    if logits.dtype != torch.float32 or logits.dim() != 3 or logits.stride(2) != 1 or logits.shape[1] < 1 or logits.shape[2] < 1:
+        raise KernelError("verify_drafts: logits are float32 [batch, drafts + 1, vocab] with unit inner stride")
+    b, g, vocab = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    temperature, top_k = float(temperature), max(int(top_k), 0)
+    if temperature != temperature or temperature == float("inf"):
+        raise KernelError(f"verify_drafts: the temperature is a finite number, got {temperature}")
+    greedy = temperature <= 0.0 or top_k == 1
+    if draft_logits is not None and (draft_logits.dtype != torch.float32 or tuple(draft_logits.shape) != (b, g, vocab)
+                                     or (g > 0 and draft_logits.stride(2) != 1)):
+        raise KernelError(f"verify_drafts: the draft's logits are float32 [{b}, {g}, {vocab}] with unit inner stride")
+    if draft_logits is None and not greedy and g > 0:
+        raise KernelError("verify_drafts: at a temperature the logits that the drafts were sampled from are needed")
+    _i32(drafts, "drafts")
+    if tuple(drafts.shape) != (b, g) or draws.dtype != torch.float64 or tuple(draws.shape) != (b, g + 1) or not draws.is_contiguous():
+        raise KernelError(f"verify_drafts: drafts are int32 [{b}, {g}] and draws contiguous float64 [{b}, {g + 1}]")
+    _on_current_device(logits, draft_logits, drafts, draws)
+    tokens = torch.empty((b, g + 1), dtype=torch.int32, device=logits.device)
+    kept = torch.empty((b,), dtype=torch.int32, device=logits.device)
+    if b == 0:
+        return tokens, kept
+    rows = b * (g + 1 if greedy else 2 * g + 1)
+    parts = max(1, min(16, 592 // rows, vocab // 4096))       # blocks a row: four an SM where the row is long enough
+    size = library().mu_verify_scratch(b, g, parts)
+    if size < 0:
+        raise KernelError(f"verify_drafts: {b} sequences of {g} drafts are too many")
+    scratch_ = torch.empty((size,), dtype=torch.uint8, device=logits.device)
+    q = draft_logits if g > 0 and not greedy else None
+    _check(library().mu_verify_drafts(
+        _ptr(logits), logits.stride(0), logits.stride(1), _ptr(q), q.stride(0) if q is not None else 0,
+        q.stride(1) if q is not None else 0, b, g, vocab, _ptr(drafts) if g > 0 else None, _ptr(draws), temperature, top_k, parts,
+        _ptr(scratch_), _ptr(tokens), _ptr(kept), _stream()), ("verify_drafts(drafts={}, vocab={})", g, vocab), launches=2)
+    return tokens, kept
 
 
 class NormedInput:

@@ -1,0 +1,289 @@
+// Rows and weights in 8 and 4 bits with a power-of-two scale for every 32 entries (block_scaled.cuh).
+//
+// mu_quantize_q4          a weight matrix to e2m1 codes and exponent bytes.
+// mu_quantize_q8          rows to e4m3 codes and exponent bytes; with two pieces, bfloat16 rows to codes that together hold
+//                         them exactly.
+// mu_residual_add_norm_q8 x += (mult * y + mult2 * y2) * scale on the float32 stream, then h = x / sqrt(mean(x^2) + eps) *
+//                         weight, written in 8 bits.
+//
+// What bounds them is bytes: the norm reads 8 and writes 4 + 1 + 1/32 for an entry.
+#include "addend.cuh"
+#include "block_scaled.cuh"
+
+namespace mu {
+
+__device__ __forceinline__ float group_max(float top) {           // over the four lanes that hold a group, eight entries each
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) top = larger_magnitude(top, __shfl_xor_sync(0xffffffffu, top, o));
+    return top;
+}
+__device__ __forceinline__ float max_of_eight(const float (&v)[8]) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = larger_magnitude(top, v[i]);
+    return top;
+}
+
+// Eight entries of a row from column c on; columns from k on are zeros.
+template <bool VEC, typename TE>
+__device__ __forceinline__ void load_eight(const TE* row, int c, int k, float (&v)[8]) {
+    if (VEC) {
+        if (c >= k) {                                              // (k is a multiple of eight then)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        } else if (sizeof(TE) == 2) {
+            const uint4 raw = *reinterpret_cast<const uint4*>(row + c);
+            const unsigned int w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+            }
+        } else {
+            const float4 a = *reinterpret_cast<const float4*>(row + c), b = *reinterpret_cast<const float4*>(row + c + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < k ? to_float(row[c + i]) : 0.0f;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- weights
+// A thread a group.  The exponent is the smallest at which no entry is cut off at 6, or the one below it where that leaves
+// the smaller sum of squared errors (most entries gain a bit, the largest is cut).
+__device__ __forceinline__ float e2m1_error(const float (&v)[32], int b) {
+    const float f = inverse_scale(b), s = scale_value(b);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const __nv_fp4x2_storage_t c = __nv_cvt_float2_to_fp4x2(make_float2(v[2 * i] * f, v[2 * i + 1] * f), __NV_E2M1, cudaRoundNearest);
+        const float2 back = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2(c, __NV_E2M1)));
+        const float d0 = (back.x - v[2 * i] * f), d1 = (back.y - v[2 * i + 1] * f);
+        sum = fmaf(d0, d0, fmaf(d1, d1, sum));
+    }
+    return sum * s * s;
+}
+
+template <typename TE>
+__global__ void __launch_bounds__(128)
+quantize_q4_kernel(const TE* __restrict__ w, long long ldw, int n, int k, int kp, unsigned char* __restrict__ codes,
+                   unsigned char* __restrict__ scales) {
+    const int groups = kp / BS_GROUP;
+    const long long item = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    const long long row = item / groups;
+    const int g = (int)(item % groups);
+    const long long rows = ((long long)n + BS_TILE - 1) / BS_TILE * BS_TILE;
+    if (row >= rows) return;
+    unsigned char* at = scales + scale_at(row, g, kp / BS_TILE);
+    if (row >= n) {                                                // the tile's rows past the matrix: a scale, no codes
+        *at = 0;
+        return;
+    }
+    float v[32];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const int c = g * BS_GROUP + i;
+        v[i] = c < k ? to_float(w[row * ldw + c]) : 0.0f;
+        top = larger_magnitude(top, v[i]);
+    }
+    uint4 packed = make_uint4(0, 0, 0, 0);
+    int b = 255;                                                   // a group holding an infinity or NaN is NaN
+    if (is_finite_magnitude(top)) {
+        b = exponent_e2m1(top);
+        if (b > 0 && e2m1_error(v, b - 1) < e2m1_error(v, b)) --b;
+        const float f = inverse_scale(b);
+        unsigned int word[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            word[i / 4] |= (unsigned int)__nv_cvt_float2_to_fp4x2(make_float2(v[2 * i] * f, v[2 * i + 1] * f), __NV_E2M1, cudaRoundNearest) << (8 * (i % 4));
+        packed = make_uint4(word[0], word[1], word[2], word[3]);
+    }
+    *reinterpret_cast<uint4*>(codes + row * (kp / 2) + (long long)g * 16) = packed;
+    *at = (unsigned char)b;
+}
+
+// ------------------------------------------------------------------------------------------------- rows
+// Eight entries a thread, four neighbouring lanes a group.  PIECES = 2: the second piece's codes lie `rows x kp` bytes, its
+// exponents a whole set of tiles, behind the first's.
+template <typename TE, int PIECES, bool VEC>
+__global__ void __launch_bounds__(256)
+quantize_q8_kernel(const TE* __restrict__ x, long long ldx, int m, int k, int kp, unsigned char* __restrict__ codes,
+                   unsigned char* __restrict__ scales) {
+    pdl_trigger();
+    pdl_wait();
+    const int eights = kp / 8;
+    const long long item = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    const long long row = item / eights;
+    const int c = (int)(item % eights) * 8;
+    const long long rows = ((long long)m + BS_TILE - 1) / BS_TILE * BS_TILE;
+    const bool real = row < m;
+    float v[8];
+    if (real) load_eight<VEC>(x + row * ldx, c, k, v);
+    else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    }
+    const float top = group_max(max_of_eight(v));                  // (every lane of the warp takes part)
+    const bool fine = is_finite_magnitude(top);
+    const int b = fine ? exponent_e4m3(top) : 127;
+    if (real) {
+        uint2 hi, lo;
+        if (PIECES == 2) e4m3_pieces_of_eight(v, b, hi, lo);
+        else hi = e4m3_of_eight(v, b);
+        if (!fine) hi = lo = make_uint2(E4M3_NAN4, E4M3_NAN4);
+        *reinterpret_cast<uint2*>(codes + row * kp + c) = hi;
+        if (PIECES == 2) *reinterpret_cast<uint2*>(codes + ((long long)m + row) * kp + c) = lo;
+    }
+    if (row < rows && c % BS_GROUP == 0) {
+        unsigned char* at = scales + scale_at(row, c / BS_GROUP, kp / BS_TILE);
+        *at = (unsigned char)b;
+        if (PIECES == 2) at[rows * (kp / BS_GROUP)] = (unsigned char)low_exponent(b);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- the norm
+// A block a row, eight entries a thread and turn; up to KEEP turns stay in registers between the sum and the codes, wider
+// rows are read again from the stream (each entry by the thread that wrote it).
+template <int THREADS, int KEEP, bool VEC>
+__global__ void __launch_bounds__(THREADS)
+residual_add_norm_q8_kernel(float* __restrict__ x, long long ldx, const Addend add, const float* __restrict__ weight, float eps,
+                            int m, int width, int kp, unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
+    __shared__ float scratch[32];
+    pdl_trigger();
+    pdl_wait();
+    const long long t = blockIdx.x;
+    float* xs = x + t * ldx;
+    float kept[KEEP][8];
+    float sq = 0.0f;
+    auto take = [&](int c, float (&v)[8]) {                        // the stream's entries with the addition made
+        load_eight<VEC>(xs, c, width, v);
+        if (!add.y || c >= width) return;
+        if (VEC) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 s = ra_added4(make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]), add, t, c + 4 * h);
+                *reinterpret_cast<float4*>(xs + c + 4 * h) = s;
+                v[4 * h] = s.x; v[4 * h + 1] = s.y; v[4 * h + 2] = s.z; v[4 * h + 3] = s.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < width) { v[i] = ra_added(v[i], add, t, c + i); xs[c + i] = v[i]; }
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) {
+        const int c = 8 * (threadIdx.x + j * THREADS);
+        take(c, kept[j]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sq = fmaf(kept[j][i], kept[j][i], sq);
+    }
+    for (int c = 8 * (threadIdx.x + KEEP * THREADS); c < width; c += 8 * THREADS) {
+        float v[8];
+        take(c, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sq = fmaf(v[i], v[i], sq);
+    }
+    const float inv = 1.0f / sqrtf(block_sum(sq, scratch) / (float)width + eps);
+    auto put = [&](int c, float (&v)[8]) {                         // all four lanes of a group are here together
+        float g[8];
+        load_eight<VEC>(weight, c, width, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * g[i];
+        const float top = group_max(max_of_eight(v));
+        const bool fine = is_finite_magnitude(top);
+        const int b = fine ? exponent_e4m3(top) : 127;
+        const uint2 code = fine ? e4m3_of_eight(v, b) : make_uint2(E4M3_NAN4, E4M3_NAN4);
+        if (c < kp) {
+            *reinterpret_cast<uint2*>(codes + t * kp + c) = code;
+            if (c % BS_GROUP == 0) scales[scale_at(t, c / BS_GROUP, kp / BS_TILE)] = (unsigned char)b;
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < KEEP; ++j) put(8 * (threadIdx.x + j * THREADS), kept[j]);
+    for (int c = 8 * (threadIdx.x + KEEP * THREADS); c - 8 * (threadIdx.x & 31) < kp; c += 8 * THREADS) {
+        float v[8];
+        load_eight<VEC>(xs, c, width, v);                          // written above by this very thread
+        put(c, v);
+    }
+    // the last row's block gives the tile's rows behind it their (unused) exponents
+    if (t == m - 1) {
+        const long long behind = ((long long)m + BS_TILE - 1) / BS_TILE * BS_TILE - m;
+        const int words = kp / BS_TILE;
+        for (long long i = threadIdx.x; i < behind * words; i += THREADS)
+            *reinterpret_cast<unsigned int*>(scales + scale_at(m + i / words, (int)(i % words) * 4, words)) = 0u;
+    }
+}
+
+}  // namespace mu
+
+// w [n, k] (ldw) bfloat16 or float32 -> codes [n, kp / 2], scales [ceil(n / 128), kp / 128, 512]; kp: k rounded up to 128.
+MU_EXPORT int mu_quantize_q4(const void* w, long long ldw, int is_bf16, int n, int k, int kp, void* codes, void* scales,
+                             void* stream) {
+    if (n <= 0) return MU_OK;
+    if (!w || !codes || !scales || k <= 0 || kp % 128 || kp < k || kp - k >= 128 || ldw < k) return MU_ERR_BAD_ARGUMENT;
+    if (((uintptr_t)codes | (uintptr_t)scales) & 15) return MU_ERR_ALIGNMENT;
+    const long long rows = ((long long)n + 127) / 128 * 128, items = rows * (kp / 32);
+    const long long blocks = (items + 127) / 128;
+    if (blocks > 2147483647ll) return MU_ERR_UNSUPPORTED_SIZE;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (is_bf16)
+        mu::quantize_q4_kernel<__nv_bfloat16><<<(unsigned)blocks, 128, 0, s>>>((const __nv_bfloat16*)w, ldw, n, k, kp, (unsigned char*)codes, (unsigned char*)scales);
+    else
+        mu::quantize_q4_kernel<float><<<(unsigned)blocks, 128, 0, s>>>((const float*)w, ldw, n, k, kp, (unsigned char*)codes, (unsigned char*)scales);
+    MU_CHECK_LAUNCH();
+    return MU_OK;
+}
+
+// x [m, k] (ldx) bfloat16 or float32 -> codes [pieces, m, kp], scales [pieces, ceil(m / 128), kp / 128, 512].
+MU_EXPORT int mu_quantize_q8(const void* x, long long ldx, int is_bf16, int m, int k, int kp, int pieces, void* codes,
+                             void* scales, void* stream) {
+    if (m <= 0) return MU_OK;
+    if (!x || !codes || !scales || k <= 0 || kp % 128 || kp < k || kp - k >= 128 || (m > 1 && ldx < k) || pieces < 1 || pieces > 2 ||
+        (pieces == 2 && !is_bf16))
+        return MU_ERR_BAD_ARGUMENT;
+    if (((uintptr_t)codes | (uintptr_t)scales) & 15) return MU_ERR_ALIGNMENT;
+    const long long rows = ((long long)m + 127) / 128 * 128, items = rows * (kp / 8);
+    const long long blocks = (items + 255) / 256;
+    if (blocks > 2147483647ll) return MU_ERR_UNSUPPORTED_SIZE;
+    const bool vec = k % 8 == 0 && ((uintptr_t)x & 15) == 0 && (m == 1 || ldx % (is_bf16 ? 8 : 4) == 0);
+    cudaStream_t s = (cudaStream_t)stream;
+#define MU_Q8(TE, PIECES, VEC) \
+    return mu::launch_pdl(mu::quantize_q8_kernel<TE, PIECES, VEC>, dim3((unsigned)blocks), dim3(256), 0, s, 1, (const TE*)x, ldx, m, k, kp, \
+                          (unsigned char*)codes, (unsigned char*)scales)
+    if (pieces == 2) { if (vec) MU_Q8(__nv_bfloat16, 2, true); MU_Q8(__nv_bfloat16, 2, false); }
+    if (is_bf16) { if (vec) MU_Q8(__nv_bfloat16, 1, true); MU_Q8(__nv_bfloat16, 1, false); }
+    if (vec) MU_Q8(float, 1, true);
+    MU_Q8(float, 1, false);
+#undef MU_Q8
+}
+
+// As mu_residual_add_norm with one group, the normed rows in 8 bits: codes [m, kp], scales [ceil(m / 128), kp / 128, 512].
+MU_EXPORT int mu_residual_add_norm_q8(float* x, long long ldx, const float* y, long long ldy, float mult, const float* y2,
+                                      long long ldy2, float mult2, const float* scale, const float* weight, float eps, int m,
+                                      int width, int kp, void* codes, void* scales, void* stream) {
+    if (m <= 0) return MU_OK;
+    if (!x || !weight || !codes || !scales || width <= 0 || kp % 128 || kp < width || kp - width >= 128 || (y2 && !y) || (scale && !y))
+        return MU_ERR_BAD_ARGUMENT;
+    if (((uintptr_t)codes | (uintptr_t)scales) & 15) return MU_ERR_ALIGNMENT;
+    const mu::Addend add = {y, ldy, mult, y2, ldy2, mult2, scale};
+    const bool vec = width % 8 == 0 && ldx % 4 == 0 && ldy % 4 == 0 && ldy2 % 4 == 0 &&
+                     (((uintptr_t)x | (uintptr_t)y | (uintptr_t)y2 | (uintptr_t)scale | (uintptr_t)weight) & 15) == 0;
+    cudaStream_t s = (cudaStream_t)stream;
+#define MU_NORM8(THREADS, KEEP, VEC)                                                                                            \
+    return mu::launch_pdl(mu::residual_add_norm_q8_kernel<THREADS, KEEP, VEC>, dim3((unsigned)m), dim3(THREADS), 0, s, 1, x, ldx, add, \
+                          weight, eps, m, width, kp, (unsigned char*)codes, (unsigned char*)scales)
+    if (vec) {
+        if (kp <= 1024) MU_NORM8(128, 1, true);
+        if (kp <= 2048) MU_NORM8(256, 1, true);
+        if (kp <= 4096) MU_NORM8(256, 2, true);
+        MU_NORM8(256, 4, true);
+    }
+    if (kp <= 1024) MU_NORM8(128, 1, false);
+    if (kp <= 2048) MU_NORM8(256, 1, false);
+    MU_NORM8(256, 4, false);
+#undef MU_NORM8
+}

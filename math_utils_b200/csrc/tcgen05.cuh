@@ -148,6 +148,12 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// The driver's cuTensorMapEncodeTiled (gemm_tc.cu); null if it cannot be had.
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled_fn();
+
 // A [rows, cols] bfloat16 matrix with `ld` elements between rows, cut into boxes of box_rows x 64 with the
 // 128-byte swizzle (gemm_tc.cu; descriptors are cached by address and shape).  False if the driver refuses.
 bool tensor_map_bf16(CUtensorMap* map, const void* base, long long rows, int cols, long long ld, int box_rows);
