@@ -24,30 +24,24 @@ __host__ __device__ __forceinline__ long long scale_at(long long row, int group,
     return ((row / BS_TILE) * kb + group / 4) * BS_TILE_BYTES + (row % 32) * 16 + (row % BS_TILE) / 32 * 4 + group % 4;
 }
 
-// The exponent byte for a group whose largest magnitude is `top` (finite): the smallest b with top <= 448 * 2^(b - 127).
+// Magnitudes are compared as bit patterns without the sign: they order as the numbers do, an infinity and NaN above every one.
+__device__ __forceinline__ unsigned int magnitude_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+__device__ __forceinline__ bool is_number(unsigned int top) { return top < 0x7F800000u; }
+
+// The exponent byte for a group whose largest magnitude's pattern is `top` (a number's): the smallest b with top <= 448 * 2^(b - 127).
 // 448 = 1.75 * 2^8, so b is the exponent field of top less 8, and one more where top's mantissa is above 1.75.
-__device__ __forceinline__ int exponent_e4m3(float top) {
-    const unsigned int bits = __float_as_uint(top);
-    const int b = (int)(bits >> 23) - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+__device__ __forceinline__ int exponent_e4m3(unsigned int top) {
+    const int b = (int)(top >> 23) - 8 + ((top & 0x7FFFFFu) > 0x600000u ? 1 : 0);
     return b > 0 ? b : 0;
 }
 // The same for e2m1, whose largest value is 6 = 1.5 * 2^2.
-__device__ __forceinline__ int exponent_e2m1(float top) {
-    const unsigned int bits = __float_as_uint(top);
-    const int b = (int)(bits >> 23) - 2 + ((bits & 0x7FFFFFu) > 0x400000u ? 1 : 0);
+__device__ __forceinline__ int exponent_e2m1(unsigned int top) {
+    const int b = (int)(top >> 23) - 2 + ((top & 0x7FFFFFu) > 0x400000u ? 1 : 0);
     return b > 0 ? (b < 254 ? b : 254) : 0;
 }
 // 2^(127 - b), by which a group's entries are multiplied on the way to their codes (exact: a power of two).
 __device__ __forceinline__ float inverse_scale(int b) { return __uint_as_float((unsigned int)(254 - b) << 23); }
 __device__ __forceinline__ float scale_value(int b) { return b > 0 ? __uint_as_float((unsigned int)b << 23) : __uint_as_float(0x00400000u); }
-
-__device__ __forceinline__ bool is_finite_magnitude(float top) { return __float_as_uint(top) < 0x7F800000u; }
-// The larger magnitude; NaN where either is NaN (so that a group holding one is seen).
-__device__ __forceinline__ float larger_magnitude(float a, float b) {
-    a = fabsf(a);
-    b = fabsf(b);
-    return (a > b || a != a) ? a : b;
-}
 
 __device__ __forceinline__ unsigned int e4m3_pair(float lo, float hi) {
     return (unsigned int)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
@@ -73,19 +67,36 @@ __device__ __forceinline__ uint2 e4m3_of_eight(const float (&v)[8], int b) {
 // 2^-4 of v that is a multiple of 2^-7 of v's leading bit: 4 bits, which lo holds exactly.  (Entries below 2^-14 of the
 // group's largest lose what lies below 2^-22 of that largest one.)  The exponent byte of lo is b - 4; where b < 4 (a
 // group below 2^-115) its scale stays at 2^-127 and lo is made for that scale.
+//
+// words: the entries as they lie in memory, two a word.
 __device__ __forceinline__ int low_exponent(int b) { return b > 4 ? b - 4 : 0; }
-__device__ __forceinline__ void e4m3_pieces_of_eight(const float (&v)[8], int b, uint2& hi, uint2& lo) {
-    const float s = scale_value(b), fl = inverse_scale(low_exponent(b));
-    hi = e4m3_of_eight(v, b);
-    float r[8];
+__device__ __forceinline__ void e4m3_pieces_of_eight(const unsigned int (&words)[4], int b, uint2& hi, uint2& lo) {
+    const float f = inverse_scale(b);
+    const float up = b > 4 ? 16.0f : __uint_as_float((unsigned int)(127 + b) << 23);      // 2^(scale of hi - scale of lo)
+    unsigned int h[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 h = of_e4m3_pair(((i < 2 ? hi.x : hi.y) >> (16 * (i & 1))) & 0xFFFFu);
-        r[2 * i] = (v[2 * i] - h.x * s) * fl;
-        r[2 * i + 1] = (v[2 * i + 1] - h.y * s) * fl;
+        const float v0 = __uint_as_float(words[i] << 16) * f, v1 = __uint_as_float(words[i] & 0xFFFF0000u) * f;
+        h[i] = e4m3_pair(v0, v1);
+        const float2 back = of_e4m3_pair(h[i]);
+        l[i] = e4m3_pair((v0 - back.x) * up, (v1 - back.y) * up);
     }
-    lo.x = e4m3_pair(r[0], r[1]) | e4m3_pair(r[2], r[3]) << 16;
-    lo.y = e4m3_pair(r[4], r[5]) | e4m3_pair(r[6], r[7]) << 16;
+    hi = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    lo = make_uint2(l[0] | l[1] << 16, l[2] | l[3] << 16);
+}
+
+// The largest magnitude of the group that four neighbouring lanes hold, eight bfloat16 each (two a word), as its bit pattern
+// without the sign: patterns order as magnitudes do, an infinity and NaN above every number.
+__device__ __forceinline__ unsigned int group_top_bf16(const unsigned int (&words)[4]) {
+    unsigned int top = __vmaxu2(__vmaxu2(words[0] & 0x7FFF7FFFu, words[1] & 0x7FFF7FFFu), __vmaxu2(words[2] & 0x7FFF7FFFu, words[3] & 0x7FFF7FFFu));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    return max(top & 0xFFFFu, top >> 16);
+}
+// exponent_e4m3 of a bfloat16's pattern, and whether it is a number's.
+__device__ __forceinline__ int exponent_e4m3_bf16(unsigned int top) {
+    const int b = (int)(top >> 7) - 8 + ((top & 0x7Fu) > 0x60u ? 1 : 0);
+    return b > 0 ? b : 0;
 }
 
 }  // namespace mu

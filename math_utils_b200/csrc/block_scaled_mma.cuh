@@ -27,13 +27,16 @@ __device__ __forceinline__ void umma_block_scaled(uint32_t tmem_d, uint64_t desc
 
 // A tile of exponent bytes (512 bytes: 32 rows of 16) from shared memory to four columns of tensor memory, the same in
 // each quarter of its lanes.  In order with the products issued after it by the same thread.
-__device__ __forceinline__ void copy_scales(uint32_t tmem_dst, uint32_t smem_addr) {
+__device__ __forceinline__ uint64_t scales_desc(uint32_t smem_addr) {
     uint64_t d = 0;                                     // no swizzle: 8 rows of 16 bytes one after another, groups 128 bytes apart
     d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
     d |= (uint64_t)1 << 16;
     d |= (uint64_t)(128 >> 4) << 32;
     d |= (uint64_t)1 << 46;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem_dst), "l"(d) : "memory");
+    return d;
+}
+__device__ __forceinline__ void copy_scales(uint32_t tmem_dst, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem_dst), "l"(desc) : "memory");
 }
 
 // `bytes` (a multiple of 16) from global to shared memory, both 16-byte aligned.
@@ -47,5 +50,7 @@ __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint3
 bool tensor_map_q4(CUtensorMap* map, const void* base, long long rows, int kp, int box_rows);
 // Codes of rows [m, kp bytes] in boxes of box_rows x 128.
 bool tensor_map_q8(CUtensorMap* map, const void* base, long long rows, int kp, int box_rows);
+// As tensor_map_out, made anew.
+bool tensor_map_boxes(CUtensorMap* map, const void* base, long long rows, int cols, long long ld, int is_bf16);
 
 }  // namespace mu

@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 import threading
 from typing import NamedTuple, Optional
 
@@ -188,17 +189,22 @@ _SIGNATURES = {
     "mu_rms_norm_pair": [_c_p, _c_ll, _c_p, _c_p, _c_f, _c_p, _c_ll, _c_p, _c_ll, _c_int, _c_int, _c_int, _c_p],
     "mu_softcap": [_c_p, _c_ll, _c_int, _c_int, _c_f, _c_p],
     "mu_moe_tile_rows": [],
-    "mu_verify_scratch": [_c_int] * 3,
-    "mu_verify_drafts": [_c_p, _c_ll, _c_ll, _c_p, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_p, _c_p, ctypes.c_double, _c_int,
-                         _c_int, _c_p, _c_p, _c_p, _c_p],
+    "mu_verify_drafts": [ctypes.c_char_p],
+    "mu_verify_args_size": [],
     "mu_quantize_q4": [_c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p, _c_p],
-    "mu_quantize_q8": [_c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p, _c_p],
-    "mu_residual_add_norm_q8": [_c_p, _c_ll, _c_p, _c_ll, _c_f, _c_p, _c_ll, _c_f, _c_p, _c_p, _c_f, _c_int, _c_int, _c_int,
-                                _c_p, _c_p, _c_p],
-    "mu_q4_few_rows": [_c_p] * 8 + [_c_p, _c_int, _c_int, _c_int, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_p, _c_p],
-    "mu_sample": [_c_p, _c_ll, _c_int, _c_int, _c_f, _c_int, _c_ull, _c_p, _c_p, _c_p, _c_p, _c_p, _c_int,
-                  _c_p, _c_p, _c_p],
+    "mu_quantize_q8": [_c_p, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_p, _c_p, _c_p],
+    "mu_residual_add_norm_q8": [ctypes.c_char_p],
+    "mu_linear_q4": [ctypes.c_char_p],
+    "mu_norm_q8_args_size": [],
+    "mu_linear_q4_args_size": [],
 }
+
+
+# Arguments that go to the library as one record (LinearQ4Args in q4_linear.cu, NormQ8Args in q8_rows.cu, VerifyArgs in verify.cu):
+# twenty arguments one by one cost 1.9 us of the host, packed 0.4.
+_LINEAR_Q4_ARGS = struct.Struct("10P3q8i")
+_NORM_Q8_ARGS = struct.Struct("8P3q3f3i")
+_VERIFY_ARGS = struct.Struct("8P4qd6i")
 
 
 def library() -> ctypes.CDLL:
@@ -219,6 +225,9 @@ def library() -> ctypes.CDLL:
                         continue          # optional kernels are looked up where they are used
                     fn.argtypes = argtypes
                     fn.restype = _c_int
+                if (lib.mu_linear_q4_args_size() != _LINEAR_Q4_ARGS.size or lib.mu_norm_q8_args_size() != _NORM_Q8_ARGS.size
+                        or lib.mu_verify_args_size() != _VERIFY_ARGS.size):
+                    raise KernelError("the packed arguments of the Python side and of the kernel library differ")
                 if not PDL:
                     lib.mu_set_pdl(0)         # plain stream order between kernels
                 _lib = lib
@@ -1740,15 +1749,28 @@ def _padded(k: int) -> int:
 
 def _on_current_device(*tensors) -> None:
     """These kernels are launched on the current device's stream: tensors of another device are refused."""
-    _need_cuda(*tensors)
-    current = _current_device() if _current_device is not None else torch.cuda.current_device()
+    device = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.get_device() != current:
-            raise KernelError(f"a tensor lies on {t.device}, the current device is cuda:{current}")
+        if t is not None and (t.get_device() != device or device < 0):
+            _need_cuda(*tensors)
+            raise KernelError(f"tensors lie on {tensors[0].device} and on {t.device}")
+    if device != (torch.cuda.current_device() if _current_device is None else _current_device()):
+        raise KernelError(f"the tensors lie on cuda:{device}, which is not the current device")
 
 
-def _scales_for(rows: int, kp: int, device) -> torch.Tensor:
-    return torch.empty((-(-rows // 128), kp // 128, 32, 4, 4), dtype=torch.float8_e8m0fnu, device=device)
+_empties = {}          # by dtype and device: a tensor without entries, whose new_empty is the shortest way to memory
+
+
+def _new(like: torch.Tensor, dtype: torch.dtype, *shape: int) -> torch.Tensor:
+    key = (dtype, like.get_device())
+    e = _empties.get(key)
+    if e is None:
+        e = _empties[key] = torch.empty(0, dtype=dtype, device=like.device)
+    return e.new_empty(*shape)
+
+
+def _scales_for(like: torch.Tensor, rows: int, kp: int) -> torch.Tensor:
+    return _new(like, torch.float8_e8m0fnu, -(-rows // 128), kp // 128, 32, 4, 4)
 
 
 def _check_scaled(codes: torch.Tensor, scales: torch.Tensor, kp: int, what: str) -> None:
@@ -1769,8 +1791,7 @@ def quantize_q4(w: torch.Tensor) -> Q4Weight:
     _on_current_device(w)
     n, k = w.shape
     kp = _padded(k)
-    codes = torch.empty((n, kp // 2), dtype=torch.uint8, device=w.device)
-    scales = _scales_for(n, kp, w.device)
+    codes, scales = _new(w, torch.uint8, n, kp // 2), _scales_for(w, n, kp)
     _check(library().mu_quantize_q4(_ptr(w), w.stride(0) if n > 1 else k, is_bf16, n, k, kp, _ptr(codes), _ptr(scales), _stream()),
            ("quantize_q4({}x{})", n, k))
     return Q4Weight(codes, scales)
@@ -1786,9 +1807,8 @@ def quantize_q8(x: torch.Tensor) -> Q8Rows:
     _on_current_device(x)
     m, k = x.shape
     kp = _padded(k)
-    codes = torch.empty((m, kp), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = _scales_for(m, kp, x.device)
-    _check(library().mu_quantize_q8(_ptr(x), x.stride(0), is_bf16, m, k, kp, 1, _ptr(codes), _ptr(scales), _stream()),
+    codes, scales = _new(x, torch.float8_e4m3fn, m, kp), _scales_for(x, m, kp)
+    _check(library().mu_quantize_q8(_ptr(x), x.stride(0), is_bf16, m, k, kp, _ptr(codes), _ptr(scales), _stream()),
            ("quantize_q8({}x{})", m, k))
     return Q8Rows(codes, scales)
 
@@ -1811,76 +1831,76 @@ def residual_add_norm_q8(x: torch.Tensor, y: Optional[torch.Tensor], mult: float
         raise KernelError("residual_add_norm_q8: a contiguous float32 weight of n values")
     _on_current_device(x, y, weight, y2, scale)
     kp = _padded(k)
-    codes = torch.empty((m, kp), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = _scales_for(m, kp, x.device)
-    _check(library().mu_residual_add_norm_q8(
-        x.data_ptr(), x.stride(0), _ptr(y), y.stride(0) if y is not None else 0, mult, _ptr(y2),
-        y2.stride(0) if y2 is not None else 0, mult2, _ptr(scale), weight.data_ptr(), eps, m, k, kp, codes.data_ptr(),
-        scales.data_ptr(), _stream()), ("residual_add_norm_q8(n={})", k))
+    codes, scales = _new(x, torch.float8_e4m3fn, m, kp), _scales_for(x, m, kp)
+    _check(library().mu_residual_add_norm_q8(_NORM_Q8_ARGS.pack(
+        x.data_ptr(), 0 if y is None else y.data_ptr(), 0 if y2 is None else y2.data_ptr(), 0 if scale is None else scale.data_ptr(),
+        weight.data_ptr(), codes.data_ptr(), scales.data_ptr(), _stream(), x.stride(0), 0 if y is None else y.stride(0),
+        0 if y2 is None else y2.stride(0), mult, mult2, eps, m, k, kp)), ("residual_add_norm_q8(n={})", k))
     return Q8Rows(codes, scales)
+
+
+# bfloat16 rows beyond this many need room for their pieces (Q4_CUT_INSIDE in q4_linear.cu: up to it the product's own blocks cut them;
+# 16 x 6,400 x 1,600: 7.4 us in one launch and 9 in two; 32 x 11,264 x 2,048: 16 and 12)
+_Q4_CUT_INSIDE = 16
 
 
 def linear_q4(x, weight: Q4Weight, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
               residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-              out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+              out_dtype: Optional[torch.dtype] = None, way: int = 0) -> torch.Tensor:
     """act(x @ W^T + bias) + residual with W in 4 bits.  ``x``: bfloat16 [m, k] with unit stride along k (taken as they
     are: cut into two 8-bit pieces that together hold them), ``Q8Rows``, or a ``NormedInput``.  Sums are float32;
     ``out`` bfloat16 (the default) or float32; ``bias`` float32 [n], ``residual`` float32 [m, n], which may be ``out``.
-    A row that holds an infinity or NaN gives NaN."""
+    A row that holds an infinity or NaN gives NaN.  ``way``: 0, or which kernel runs: 1 + b the one for few rows (up to
+    64) with b blocks a tile (0: the library chooses), -64, -128 or -192 the one for many with tiles that wide."""
     if isinstance(x, NormedInput):
         x = x.materialize()
     codes, w_scales = weight
-    if codes.dtype != torch.uint8 or codes.dim() != 2 or codes.shape[0] < 1 or codes.shape[1] % 64 or codes.shape[1] == 0:
-        raise KernelError(f"linear_q4: the weight's codes are uint8 [n, kp / 2] with kp a multiple of 128, got {codes.dtype} {tuple(codes.shape)}")
-    n, kp = codes.shape[0], codes.shape[1] * 2
+    if codes.dtype != torch.uint8 or codes.dim() != 2:
+        raise KernelError(f"linear_q4: the weight's codes are uint8 [n, kp / 2], got {codes.dtype} {tuple(codes.shape)}")
+    n, half = codes.shape
+    kp = 2 * half
+    if n < 1 or half < 64 or half % 64:
+        raise KernelError(f"linear_q4: the weight's codes are uint8 [n, kp / 2] with kp a multiple of 128, got {tuple(codes.shape)}")
     _check_scaled(codes, w_scales, kp, "linear_q4, weight")
-    rows = isinstance(x, Q8Rows)
-    if rows:
-        x_codes, x_scales = x
-        if x_codes.dtype != torch.float8_e4m3fn or x_codes.dim() != 2 or x_codes.shape[1] != kp:
-            raise KernelError(f"linear_q4: rows are float8_e4m3fn [m, {kp}], got {x_codes.dtype} {tuple(x_codes.shape)}")
-        _check_scaled(x_codes, x_scales, kp, "linear_q4, rows")
-        m, k = x_codes.shape[0], kp
+    if type(x) is Q8Rows:
+        given, x_scales = x
+        if given.dtype != torch.float8_e4m3fn or given.dim() != 2 or given.shape[1] != kp:
+            raise KernelError(f"linear_q4: rows are float8_e4m3fn [m, {kp}], got {given.dtype} {tuple(given.shape)}")
+        _check_scaled(given, x_scales, kp, "linear_q4, rows")
+        m, k, ldx = given.shape[0], kp, 0
     else:
+        given, x_scales = x, None
         if x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1 or not 0 <= kp - x.shape[1] < 128:
             raise KernelError(f"linear_q4: rows are bfloat16 [m, k] with unit stride along k and k rounded up to 128 equal to "
                               f"{kp}, or Q8Rows; got {x.dtype} {tuple(x.shape)}")
-        x_codes = x
         m, k = x.shape
-    if act not in ACT_CODES:
+        ldx = x.stride(0)
+    code = ACT_CODES.get(act)
+    if code is None:
         raise KernelError(f"linear_q4: the activation is one of {', '.join(str(a) for a in ACT_CODES)}, got {act}")
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype or torch.bfloat16, device=codes.device)
+        out = _new(codes, torch.bfloat16 if out_dtype is None else out_dtype, m, n)
     elif out.shape != (m, n) or out.stride(1) != 1 or (out_dtype is not None and out.dtype != out_dtype):
         raise KernelError("gemm output has the wrong shape, stride or dtype")
     out_bf16 = _is_bf16(out)
     if bias is not None and (bias.dtype != torch.float32 or bias.numel() != n or not bias.is_contiguous()):
         raise KernelError("gemm bias must be contiguous float32 of length n")
-    if residual is not None and (residual.dtype != torch.float32 or residual.shape != out.shape or residual.stride(1) != 1):
-        raise KernelError("gemm residual must be float32 [m, n]")
-    _on_current_device(x_codes, codes, w_scales, bias, residual, out, x_scales if rows else None)
+    ldr = 0
+    if residual is not None:
+        if residual.dtype != torch.float32 or residual.shape != out.shape or residual.stride(1) != 1:
+            raise KernelError("gemm residual must be float32 [m, n]")
+        ldr = residual.stride(0)
+    _on_current_device(codes, w_scales, given, x_scales, out, bias, residual)
     if m == 0:
         return out
-    lib, stream = library(), _stream()
-    if rows:
-        at = (x_codes.data_ptr(), x_scales.data_ptr(), None, None)
-        step, tile = kp, kp * 4
-    else:
-        # both pieces' codes, then both pieces' exponents (whole tiles of 128 rows)
-        tiles = -(-m // 128) * (kp * 4)
-        room = torch.empty((2 * m * kp + 2 * tiles,), dtype=torch.uint8, device=codes.device)
-        first = room.data_ptr()
-        _check(lib.mu_quantize_q8(x.data_ptr(), x.stride(0), 1, m, k, kp, 2, first, first + 2 * m * kp, stream), ("quantize_q8({}x{})", m, k))
-        at = (first, first + 2 * m * kp, first + m * kp, first + 2 * m * kp + tiles)
-        step, tile = kp, kp * 4
-    ldr = residual.stride(0) if residual is not None else 0
-    for r0 in range(0, m, 128):
-        here = [None if p is None else p + (r0 * step if i % 2 == 0 else r0 // 128 * tile) for i, p in enumerate(at)]
-        _check(lib.mu_q4_few_rows(
-            *here, codes.data_ptr(), w_scales.data_ptr(), _ptr(bias),
-            None if residual is None else residual.data_ptr() + r0 * ldr * 4, out.data_ptr() + r0 * out.stride(0) * out.element_size(),
-            min(m - r0, 128), n, kp, out.stride(0), ldr, ACT_CODES[act], out_bf16, 0, status_word(codes.device).data_ptr(), stream),
-            ("linear_q4({}x{}x{})", m, n, kp))
+    room = None
+    if x_scales is None and (m > _Q4_CUT_INSIDE or way < 0):
+        room = _new(codes, torch.uint8, 2 * m * kp + 2 * (-(-m // 128) * (kp * 4)))
+    _check(library().mu_linear_q4(_LINEAR_Q4_ARGS.pack(
+        given.data_ptr(), 0 if x_scales is None else x_scales.data_ptr(), codes.data_ptr(), w_scales.data_ptr(),
+        0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), out.data_ptr(),
+        0 if room is None else room.data_ptr(), status_word(codes.device).data_ptr(), _stream(), ldx, out.stride(0), ldr, m, n, k, kp, code,
+        out_bf16, way, 0)), ("linear_q4({}x{}x{})", m, n, k), launches=1 if room is None else 2)
     return out
 
 
@@ -1987,6 +2007,9 @@ def sample(logits: torch.Tensor, temperature: float, top_k: int, seed: int,
     return out
 
 
+VERIFY_PART_BYTES = 24         # VerifyPart in verify.cu
+
+
 def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], drafts: torch.Tensor, draws: torch.Tensor,
                   temperature: float, top_k: int):
     """Which drafted tokens the target takes: (tokens int32 [batch, drafts + 1], kept int32 [batch]).
@@ -2018,21 +2041,17 @@ def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], dr
     if tuple(drafts.shape) != (b, g) or draws.dtype != torch.float64 or tuple(draws.shape) != (b, g + 1) or not draws.is_contiguous():
         raise KernelError(f"verify_drafts: drafts are int32 [{b}, {g}] and draws contiguous float64 [{b}, {g + 1}]")
     _on_current_device(logits, draft_logits, drafts, draws)
-    tokens = torch.empty((b, g + 1), dtype=torch.int32, device=logits.device)
-    kept = torch.empty((b,), dtype=torch.int32, device=logits.device)
+    tokens, kept = _new(logits, torch.int32, b, g + 1), _new(logits, torch.int32, b)
     if b == 0:
         return tokens, kept
     rows = b * (g + 1 if greedy else 2 * g + 1)
     parts = max(1, min(16, 592 // rows, vocab // 4096))       # blocks a row: four an SM where the row is long enough
-    size = library().mu_verify_scratch(b, g, parts)
-    if size < 0:
-        raise KernelError(f"verify_drafts: {b} sequences of {g} drafts are too many")
-    scratch_ = torch.empty((size,), dtype=torch.uint8, device=logits.device)
+    room = _new(logits, torch.uint8, rows * parts * VERIFY_PART_BYTES)
     q = draft_logits if g > 0 and not greedy else None
-    _check(library().mu_verify_drafts(
-        _ptr(logits), logits.stride(0), logits.stride(1), _ptr(q), q.stride(0) if q is not None else 0,
-        q.stride(1) if q is not None else 0, b, g, vocab, _ptr(drafts) if g > 0 else None, _ptr(draws), temperature, top_k, parts,
-        _ptr(scratch_), _ptr(tokens), _ptr(kept), _stream()), ("verify_drafts(drafts={}, vocab={})", g, vocab), launches=2)
+    _check(library().mu_verify_drafts(_VERIFY_ARGS.pack(
+        logits.data_ptr(), 0 if q is None else q.data_ptr(), drafts.data_ptr(), draws.data_ptr(), room.data_ptr(), tokens.data_ptr(),
+        kept.data_ptr(), _stream(), logits.stride(0), logits.stride(1), 0 if q is None else q.stride(0), 0 if q is None else q.stride(1),
+        temperature, b, g, vocab, top_k, parts, 0)), ("verify_drafts(drafts={}, vocab={})", g, vocab), launches=2)
     return tokens, kept
 
 

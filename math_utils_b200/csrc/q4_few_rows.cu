@@ -1,4 +1,4 @@
-// C[M, N] = act(X[M, K] . W[N, K]^T + bias) (+ residual) for up to 128 rows, W in 4 bits, X in 8 bits (block_scaled.cuh),
+// C[M, N] = act(X[M, K] . W[N, K]^T + bias) (+ residual) for up to 64 rows, W in 4 bits, X in 8 bits (block_scaled.cuh),
 // the WEIGHTS as the 128-row operand of tcgen05.mma and the batch as its narrow side.
 //
 // A step of single tokens reads each weight once, 17 bytes for 32 of them, and does almost no arithmetic.  The codes go
@@ -6,20 +6,26 @@
 // instruction multiplies e2m1 by e4m3 and applies both exponents.  Expanding 4-bit codes in registers would cost two
 // instructions a code where an SM takes in 46 codes a clock.
 //   * a tile is 128 rows of W (128 output columns) by all M rows of X: D[128, NB] = W_tile . X^T, NB = M rounded up to 16,
-//     32, 64 or 128; a stage is 128 of k: 8 KB of codes, 512 bytes of exponents, and the rows' share;
-//   * K is cut over the blocks of a cluster (up to 16) so that tiles x splits fill the SMs; the partial tiles meet in
-//     distributed shared memory and are added in rank order (as in gemm_rows.cu);
-//   * bfloat16 rows come as two pieces, each e4m3, that together hold them exactly: two products a step into one
-//     accumulator.
-// Warp 0 issues the copies, warp 1 owns the tensor memory and issues the products, warps 2-5 read the accumulators.
+//     32 or 64; a stage is 128 of k: 8 KB of codes, 512 bytes of exponents, and the rows' share;
+//   * K is cut over the blocks of a cluster (any number up to 8) so that tiles x splits fill the SMs; the partial tiles
+//     meet in distributed shared memory and are added in rank order.  They lie on the stages, which nothing reads once
+//     every block of the cluster has its accumulator;
+//   * bfloat16 rows are two pieces, each e4m3, that together hold them exactly: two products a step into one
+//     accumulator.  Up to 16 rows are cut here, by eight warps, two a stage (every block cuts its own share of k: 1.3 us a
+//     launch at 8 rows where a launch before costs 3); more rows come cut by a launch of their own (q8_rows.cu).
+//   * the blocks of a tile begin at different places of k (each tile one 128 further on): every block reads the same rows,
+//     and blocks in step would all ask for the same lines at once.
+// Warp 0 copies the weights, warp 6 the rows (or warps 2-9 cut them), warp 1 owns the tensor memory and issues the products,
+// warps 2-5 read the accumulators.
 // Waits are bounded as everywhere: one that runs out sets the status word, and the blocks leave together.
 #include "block_scaled_mma.cuh"
 
 namespace mu {
 
-constexpr int QF_THREADS = 192;
+constexpr int QF_THREADS = 224, QF_THREADS_CUT = 320;
 constexpr int QF_BN = 128, QF_BK = 128;
-constexpr int QF_MAX_SPLIT = 16;
+constexpr int QF_MAX_SPLIT = 8;               // blocks of a cluster
+constexpr int QF_MAX_CUT = 16;                // bfloat16 rows that are cut here
 constexpr uint32_t QF_W_BYTES = QF_BN * QF_BK;            // in shared memory: a byte a code
 constexpr uint32_t QF_W_COPIED = QF_BN * QF_BK / 2;       // what the copy of them counts on its barrier: the packed codes
 
@@ -45,30 +51,60 @@ template <int COUNT> __device__ __forceinline__ void qf_load_columns(uint32_t ta
     }
 }
 
-__device__ __forceinline__ float qf_act(float x, int act, bool to_bf16) { return to_bf16 ? apply_act_bf16(x, act) : apply_act(x, act); }
+template <int ACT> __device__ __forceinline__ float qf_act(float x, bool to_bf16) { return to_bf16 ? apply_act_bf16(x, ACT) : apply_act(x, ACT); }
 
-struct QfRows {                       // the rows' codes and exponents: one piece, or two
-    const unsigned char* scales[2];   // [tiles of 128 rows][kb][512]
+// The activation is the same for a whole launch: f(the activation as a constant), outside the loops over the elements (inside
+// them every activation is evaluated for every element: 75 cycles a row and warp).
+template <int A> struct QfAct { static constexpr int value = A; };
+template <typename F> __device__ __forceinline__ void qf_with_act(int act, F f) {
+    if (act == ACT_GELU_NEW) f(QfAct<ACT_GELU_NEW>());
+    else if (act == ACT_GELU_ERF) f(QfAct<ACT_GELU_ERF>());
+    else if (act == ACT_RELU2) f(QfAct<ACT_RELU2>());
+    else f(QfAct<ACT_NONE>());
+}
+
+// How the rows come: in 8 bits, as two pieces of a launch before, or in bfloat16 and cut into two pieces here.
+constexpr int QF_EIGHT = 0, QF_PIECES = 1, QF_SIXTEEN = 2;
+
+struct QfRows {
+    const unsigned char* scales[2];   // of the rows or their pieces: [tiles of 128 rows][kb][512]
+    const __nv_bfloat16* x;           // QF_SIXTEEN: [M, K] (ldx)
+    long long ldx;
+    int K, vec;                       // vec: rows in whole, aligned 16-byte pieces
 };
 
+// Eight bfloat16 of a row from column c on; columns from K on are zeros.
+__device__ __forceinline__ uint4 qf_load_eight(const QfRows& rows, int row, int c) {
+    const __nv_bfloat16* p = rows.x + (long long)row * rows.ldx + c;
+    if (rows.vec) return c < rows.K ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+    unsigned int w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned int lo = c + 2 * i < rows.K ? __bfloat16_as_ushort(p[2 * i]) : 0u;
+        const unsigned int hi = c + 2 * i + 1 < rows.K ? __bfloat16_as_ushort(p[2 * i + 1]) : 0u;
+        w[i] = lo | hi << 16;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // grid.x = tiles * splits: the blocks of a cluster (along x) share a tile and cut K.  Dynamic shared memory, 1,024-byte
-// aligned: per stage W 16 KB and PIECES x (NB x 128 bytes), then per stage the exponents (512 bytes each), then, with
-// splits > 1, the shares this block is sent and its own partial tile (on the stages, when they are no longer read).
-template <int NB, int PIECES, typename TC>
-__global__ void __launch_bounds__(QF_THREADS)
+// aligned: per stage W 16 KB and PIECES x (NB x 128 bytes), then per stage the exponents (512 bytes each).  With splits > 1
+// this block's partial tile and the shares it is sent lie on the stages when they are no longer read.
+template <int NB, int MODE, typename TC>
+__global__ void __launch_bounds__(MODE == QF_SIXTEEN ? QF_THREADS_CUT : QF_THREADS)
 q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x0,
                    const __grid_constant__ CUtensorMap map_x1, const unsigned char* __restrict__ w_scales, const QfRows rows,
                    const float* __restrict__ bias, const float* residual, TC* C, int M, int N, int kb_all, long long ldc,
                    long long ldr, int act, int* status, int splits, int stages) {
+    constexpr int PIECES = MODE == QF_EIGHT ? 1 : 2;
     constexpr uint32_t X_BYTES = NB * QF_BK, STAGE = QF_W_BYTES + PIECES * X_BYTES;
-    constexpr uint32_t SCALE_STAGE = (1 + PIECES) * BS_TILE_BYTES, ALL_BYTES = QF_W_COPIED + PIECES * X_BYTES + SCALE_STAGE;
+    constexpr uint32_t SCALE_STAGE = (1 + PIECES) * BS_TILE_BYTES;
     constexpr uint32_t ACC_COLS = NB < 32 ? 32 : NB, SCALE_COLS = 4 * (1 + PIECES);
-    constexpr uint32_t TMEM_COLS = ACC_COLS + 2 * SCALE_COLS <= 64 ? 64 : ACC_COLS + 2 * SCALE_COLS <= 128 ? 128 : 256;
+    constexpr uint32_t TMEM_COLS = ACC_COLS + 2 * SCALE_COLS <= 64 ? 64 : 128;
     constexpr int CHUNK = NB < 32 ? 16 : 32;
     extern __shared__ unsigned char qf_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)qf_raw + 1023) & ~(uintptr_t)1023);
     unsigned char* scale_smem = base + (size_t)stages * STAGE;
-    float* part = reinterpret_cast<float*>(scale_smem + (size_t)stages * SCALE_STAGE);
     float* outbox = reinterpret_cast<float*>(base);
     __shared__ uint64_t full[16], empty[16], acc_full, parts_in;
     __shared__ uint32_t tmem_slot;
@@ -84,9 +120,9 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 
     if (threadIdx.x == 0) {
         tma_prefetch_map(&map_w);
-        tma_prefetch_map(&map_x0);
-        if (PIECES == 2) tma_prefetch_map(&map_x1);
-        for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        if (MODE != QF_SIXTEEN) tma_prefetch_map(&map_x0);
+        if (MODE == QF_PIECES) tma_prefetch_map(&map_x1);
+        for (int s = 0; s < stages; ++s) { mbar_init(&full[s], MODE == QF_SIXTEEN ? 3 : 2); mbar_init(&empty[s], 1); }
         mbar_init(&acc_full, 1);
         mbar_init(&parts_in, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -96,7 +132,7 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                      ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (threadIdx.x >= 64) {
+    if (threadIdx.x >= 64 && threadIdx.x < 192) {
         const int n = n0 + (int)threadIdx.x - 64;
         bias_s[threadIdx.x - 64] = (bias && n < N) ? bias[n] : 0.0f;
     }
@@ -105,36 +141,42 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_acc = tmem_slot;
     pdl_trigger();
-    if (splits > 1) qf_cluster_arrive();                  // every block runs before anyone writes into another's shared memory
-
-    if (warp == 0) {
+    // The two issuing threads run alone on their warps, where every dependent instruction costs its whole latency: stages and
+    // phases are counted on instead of divided out, and addresses and descriptors are added to.  (With i % stages and
+    // descriptors made anew a stage took its loader and its issuer about 500 cycles each, more than its bytes.)
+    const int turned = tile % my_kb;                      // where this block begins in its share of k
+    if (warp == 0 || (MODE != QF_SIXTEEN && warp == 6)) {
+        const bool weights = warp == 0;
         if (lane == 0) {
-            auto load_weights = [&](int i, int s) {
-                mbar_expect_tx(&full[s], ALL_BYTES);
-                tma_load_2d(base + (size_t)s * STAGE, &map_w, (kb_begin + i) * QF_BK, n0, &full[s]);
-                bulk_load(scale_smem + (size_t)s * SCALE_STAGE, w_scales + ((long long)tile * kb_all + kb_begin + i) * BS_TILE_BYTES,
-                          BS_TILE_BYTES, &full[s]);
-            };
-            auto load_rows = [&](int i, int s) {
-#pragma unroll
-                for (int p = 0; p < PIECES; ++p) {
-                    tma_load_2d(base + (size_t)s * STAGE + QF_W_BYTES + p * X_BYTES, p == 0 ? &map_x0 : &map_x1, (kb_begin + i) * QF_BK, 0, &full[s]);
-                    bulk_load(scale_smem + (size_t)s * SCALE_STAGE + (1 + p) * BS_TILE_BYTES,
-                              rows.scales[p] + (long long)(kb_begin + i) * BS_TILE_BYTES, BS_TILE_BYTES, &full[s]);
+            int kb = turned;
+            auto load = [&](int s) {
+                const int k = kb_begin + kb;
+                if (weights) {
+                    mbar_expect_tx(&full[s], QF_W_COPIED + BS_TILE_BYTES);
+                    tma_load_2d(base + s * STAGE, &map_w, k * QF_BK, n0, &full[s]);
+                    bulk_load(scale_smem + s * SCALE_STAGE, w_scales + ((long long)tile * kb_all + k) * BS_TILE_BYTES, BS_TILE_BYTES, &full[s]);
+                } else {
+                    mbar_expect_tx(&full[s], PIECES * (X_BYTES + BS_TILE_BYTES));
+                    tma_load_2d(base + s * STAGE + QF_W_BYTES, &map_x0, k * QF_BK, 0, &full[s]);
+                    bulk_load(scale_smem + s * SCALE_STAGE + BS_TILE_BYTES, rows.scales[0] + (long long)k * BS_TILE_BYTES, BS_TILE_BYTES, &full[s]);
+                    if (MODE == QF_PIECES) {
+                        tma_load_2d(base + s * STAGE + QF_W_BYTES + X_BYTES, &map_x1, k * QF_BK, 0, &full[s]);
+                        bulk_load(scale_smem + s * SCALE_STAGE + 2 * BS_TILE_BYTES, rows.scales[1] + (long long)k * BS_TILE_BYTES, BS_TILE_BYTES, &full[s]);
+                    }
                 }
+                if (++kb == my_kb) kb = 0;
             };
+            if (!weights) pdl_wait();                     // (weights are written by no kernel)
             const int first = my_kb < stages ? my_kb : stages;
-            for (int i = 0; i < first; ++i) load_weights(i, i);      // written by no kernel: before the wait for the one before
-            pdl_wait();
-            for (int i = 0; i < first; ++i) load_rows(i, i);
-            int issued = first;
+            for (int i = 0; i < first; ++i) load(i);
+            int issued = first, s = 0;
+            uint32_t phase = 0;
             for (int i = first; i < my_kb; ++i) {
-                const int s = i % stages;
-                ok = mbar_wait(&empty[s], (uint32_t)((i / stages - 1) & 1));
+                ok = mbar_wait(&empty[s], phase);
                 if (!ok) break;
-                load_weights(i, s);
-                load_rows(i, s);
+                load(s);
                 issued = i + 1;
+                if (++s == stages) { s = 0; phase ^= 1; }
             }
             if (!ok) {
                 atomicExch(status, 1);
@@ -145,29 +187,96 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     } else if (warp == 1) {
         const bool one = elect_one();
         constexpr uint32_t idesc = idesc_block_scaled(BM_E2M1, BM_E4M3, QF_BN, NB);
+        const uint64_t w_desc0 = smem_desc_sw128(smem_u32(base)), s_desc0 = scales_desc(smem_u32(scale_smem));
+        uint64_t w_desc = w_desc0, s_desc = s_desc0;
+        int s = 0;
+        uint32_t phase = 0;
         for (int i = 0; i < my_kb; ++i) {
-            const int s = i % stages;
-            ok = mbar_wait(&full[s], (uint32_t)((i / stages) & 1));
+            ok = mbar_wait(&full[s], phase);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (!one) continue;
-            const uint32_t w_addr = smem_u32(base + (size_t)s * STAGE), s_addr = smem_u32(scale_smem + (size_t)s * SCALE_STAGE);
-            const uint32_t tmem_s = tmem_acc + ACC_COLS + (i & 1) * SCALE_COLS;      // two sets, in turn
+            if (one) {
+                const uint32_t tmem_s = tmem_acc + ACC_COLS + (i & 1) * SCALE_COLS;      // two sets, in turn
 #pragma unroll
-            for (int p = 0; p <= PIECES; ++p) copy_scales(tmem_s + 4 * p, s_addr + p * BS_TILE_BYTES);
+                for (int p = 0; p <= PIECES; ++p) copy_scales(tmem_s + 4 * p, s_desc + p * (BS_TILE_BYTES / 16));
 #pragma unroll
-            for (int j = 0; j < QF_BK / 32; ++j)
+                for (int j = 0; j < QF_BK / 32; ++j)
 #pragma unroll
-                for (int p = 0; p < PIECES; ++p)
-                    umma_block_scaled(tmem_acc, smem_desc_sw128(w_addr + j * 32), smem_desc_sw128(w_addr + QF_W_BYTES + p * X_BYTES + j * 32),
-                                      idesc | idesc_scale_byte(j), tmem_s, tmem_s + 4 + 4 * p, (i > 0 || j > 0 || p > 0) ? 1u : 0u);
-            umma_commit(&empty[s]);
+                    for (int p = 0; p < PIECES; ++p)
+                        umma_block_scaled(tmem_acc, w_desc + 2 * j, w_desc + (QF_W_BYTES + p * X_BYTES) / 16 + 2 * j,
+                                          idesc | idesc_scale_byte(j), tmem_s, tmem_s + 4 + 4 * p, (i > 0 || j > 0 || p > 0) ? 1u : 0u);
+                umma_commit(&empty[s]);
+            }
+            __syncwarp();
+            w_desc += STAGE / 16;
+            s_desc += SCALE_STAGE / 16;
+            if (++s == stages) { s = 0; phase ^= 1; w_desc = w_desc0; s_desc = s_desc0; }
         }
         if (ok && one) umma_commit(&acc_full);
         if (!ok && one) atomicExch(status, 2);
     } else {
         const int quad = warp & 3, col = quad * 32 + lane;        // a lane is an output column: n0 + col
         const bool to_bf16 = sizeof(TC) == 2;
+        if (MODE == QF_SIXTEEN) {
+            // Two warps take every fourth stage, every other pair of its rows each, a lane eight entries at a time, four neighbours
+            // a group of 32: 16 lanes a row.
+            constexpr int PAIRS = NB / 4;                          // of rows, a warp
+            const int turn = (warp - 2) & 3, pair0 = (warp - 2) >> 2;
+            const int half = lane >> 4, c8 = lane & 15;
+            pdl_wait();                                            // the rows are the work of earlier kernels
+            // Two stages' rows are on their way while a third's are cut.
+            uint4 raw[2][PAIRS];
+            auto ask = [&](int i, int e, uint4& to) {
+                const int row = 2 * (2 * e + pair0) + half;
+                to = i < my_kb && row < M ? qf_load_eight(rows, row, (kb_begin + (i + turned < my_kb ? i + turned : i + turned - my_kb)) * QF_BK + 8 * c8)
+                                          : make_uint4(0, 0, 0, 0);
+            };
+            // (a ring of four stages or more, or of all of them: a warp four stages on then waits for the phase before its own)
+            int s = turn % stages;
+            uint32_t phase = (uint32_t)(turn / stages) & 1u;
+            auto cut = [&](int i, uint4 (&mine)[PAIRS]) {
+                if (i >= stages) ok = mbar_wait(&empty[s], phase ^ 1u);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; return; }
+                unsigned char* x0 = base + s * STAGE + QF_W_BYTES;
+                unsigned char* sx = scale_smem + s * SCALE_STAGE + BS_TILE_BYTES;
+#pragma unroll
+                for (int e = 0; e < PAIRS; ++e) {
+                    if (2 * (2 * e + pair0) >= M) break;           // rows past M are left as they are: their columns go nowhere
+                    const int row = 2 * (2 * e + pair0) + half;
+                    const unsigned int w[4] = {mine[e].x, mine[e].y, mine[e].z, mine[e].w};
+                    ask(i + 8, e, mine[e]);
+                    const unsigned int top = group_top_bf16(w);
+                    const bool fine = top < 0x7F80u;
+                    const int b = fine ? exponent_e4m3_bf16(top) : 127;
+                    uint2 hi, lo;
+                    e4m3_pieces_of_eight(w, b, hi, lo);
+                    if (!fine) hi = lo = make_uint2(E4M3_NAN4, E4M3_NAN4);
+                    // the copies' layout: 16-byte pieces of a 128-byte row, swapped by the row's place among eight
+                    const int at = row * 128 + (((c8 >> 1) ^ (row & 7)) << 4) + (c8 & 1) * 8;
+                    *reinterpret_cast<uint2*>(x0 + at) = hi;
+                    *reinterpret_cast<uint2*>(x0 + X_BYTES + at) = lo;
+                    if ((c8 & 3) == 0) {
+                        const int to = (row % 32) * 16 + row / 32 * 4 + c8 / 4;
+                        sx[to] = (unsigned char)b;
+                        sx[BS_TILE_BYTES + to] = (unsigned char)low_exponent(b);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // the tensor cores read what was stored here
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[s]);
+                for (int step = 0; step < 4; ++step)
+                    if (++s == stages) { s = 0; phase ^= 1; }
+            };
+#pragma unroll
+            for (int e = 0; e < PAIRS; ++e) { ask(turn, e, raw[0][e]); ask(turn + 4, e, raw[1][e]); }
+            for (int i = turn; i < my_kb && ok; i += 8) {
+                cut(i, raw[0]);
+                if (i + 4 < my_kb && ok) cut(i + 4, raw[1]);
+            }
+            if (!ok && lane == 0) atomicExch(status, 1);
+            __syncwarp();
+        }
+        if (warp < 6) {
         ok = mbar_wait(&acc_full, 0);
         if (!ok && lane == 0) atomicExch(status, 3);
         __syncwarp();
@@ -186,19 +295,23 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                         float res[CHUNK];                         // all asked for before anything is stored: it may be C itself
 #pragma unroll
                         for (int e = 0; e < CHUNK; ++e) res[e] = (residual && c0 + e < M) ? residual[(long long)(c0 + e) * ldr + n] : 0.0f;
+                        qf_with_act(act, [&](auto a) {
 #pragma unroll
-                        for (int e = 0; e < CHUNK; ++e)
-                            if (c0 + e < M)
-                                C[(long long)(c0 + e) * ldc + n] = from_float<TC>(qf_act(__uint_as_float(r[e]) + bias_s[col], act, to_bf16) + res[e]);
+                            for (int e = 0; e < CHUNK; ++e)
+                                if (c0 + e < M)
+                                    C[(long long)(c0 + e) * ldc + n] = from_float<TC>(qf_act<decltype(a)::value>(__uint_as_float(r[e]) + bias_s[col], to_bf16) + res[e]);
+                        });
                     }
                     __syncwarp();                                 // the lanes are together for the next load
                 }
             }
         } else {
-            const int cols_per = QF_BN / splits;                  // output columns each block of the cluster finishes
+            // block r finishes the tile's columns [128 r / splits, 128 (r + 1) / splits)
+            auto first_of = [&](int r) { return QF_BN * r / splits; };
             const int groups = (M + 3) / 4;                       // batch rows travel four at a time
             const int pitch = 4 * groups + 4;
-            const uint32_t slice_bytes = (uint32_t)(cols_per * pitch) * 4u;
+            const int mine0 = first_of(rank), cols = first_of(rank + 1) - mine0;
+            float* part = outbox + (size_t)QF_BN * pitch;         // [splits][cols][pitch]: what this block is sent
             {
                 float* mine = outbox + (size_t)col * pitch;
 #pragma unroll
@@ -216,17 +329,19 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // the copies below read what was stored here
             asm volatile("bar.sync 1, 128;" ::: "memory");
             __syncwarp();
-            qf_cluster_wait();                                    // (the arrive was at the top) everyone is running
+            qf_cluster_arrive();                                  // this block's stages are no longer read ...
+            qf_cluster_wait();                                    // ... nor any other's
             if (threadIdx.x == 64) {
-                mbar_expect_tx(&parts_in, (uint32_t)(splits - 1) * slice_bytes);
+                mbar_expect_tx(&parts_in, (uint32_t)((splits - 1) * cols * pitch) * 4u);
                 for (int step = 1; step < splits; ++step) {
-                    const int owner = (rank + step) % splits;
+                    const int owner = (rank + step) % splits;     // not everyone at the same owner first
+                    const int from = first_of(owner), count = first_of(owner + 1) - from;
                     uint32_t dst, bar;
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-                                 : "=r"(dst) : "r"(smem_u32(part + (size_t)rank * cols_per * pitch)), "r"(owner));
+                                 : "=r"(dst) : "r"(smem_u32(part + (size_t)rank * count * pitch)), "r"(owner));
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&parts_in)), "r"(owner));
                     asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                                 ::"r"(dst), "r"(smem_u32(outbox + (size_t)owner * cols_per * pitch)), "r"(slice_bytes), "r"(bar)
+                                 ::"r"(dst), "r"(smem_u32(outbox + (size_t)from * pitch)), "r"((uint32_t)(count * pitch) * 4u), "r"(bar)
                                  : "memory");
                 }
             }
@@ -235,10 +350,11 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             __syncwarp();
             qf_cluster_arrive();
             pdl_wait();
-            const int who = (int)threadIdx.x - 64, total = groups * cols_per;
+            const int who = (int)threadIdx.x - 64, total = groups * cols;
+            qf_with_act(act, [&](auto a) {
             for (int idx = who; idx < total && arrived; idx += 128) {
-                const int g = idx / cols_per, i = idx - g * cols_per;
-                const int c = rank * cols_per + i, n = n0 + c;
+                const int g = idx / cols, i = idx - g * cols;
+                const int c = mine0 + i, n = n0 + c;
                 if (n >= N) continue;
                 float res[4];
 #pragma unroll
@@ -246,7 +362,7 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     res[e] = (residual && 4 * g + e < M) ? residual[(long long)(4 * g + e) * ldr + n] : 0.0f;
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 for (int r = 0; r < splits; ++r) {                // in rank order, whoever sent when
-                    const float* src = r == rank ? outbox + (size_t)c * pitch : part + ((size_t)r * cols_per + i) * pitch;
+                    const float* src = r == rank ? outbox + (size_t)c * pitch : part + ((size_t)r * cols + i) * pitch;
                     const float4 p = *reinterpret_cast<const float4*>(src + 4 * g);
                     v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
                 }
@@ -254,14 +370,17 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (4 * g + e < M)
-                        C[(long long)(4 * g + e) * ldc + n] = from_float<TC>(qf_act(out4[e] + bias_s[c], act, to_bf16) + res[e]);
+                        C[(long long)(4 * g + e) * ldc + n] = from_float<TC>(qf_act<decltype(a)::value>(out4[e] + bias_s[c], to_bf16) + res[e]);
             }
+            });
             __syncwarp();
             qf_cluster_wait();                                    // nobody leaves while a copy may still read its outbox
         }
+        }
     }
-    if (splits > 1 && warp < 2) {                                 // the same two cluster barriers as the epilogue warps
+    if (splits > 1 && (warp < 2 || warp >= 6)) {                                 // the same two cluster barriers as the epilogue warps
         __syncwarp();
+        qf_cluster_arrive();
         qf_cluster_wait();
         qf_cluster_arrive();
         qf_cluster_wait();
@@ -272,22 +391,20 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_acc), "r"(TMEM_COLS) : "memory");
 }
 
-template <int NB, int PIECES, typename TC>
+template <int NB, int MODE, typename TC>
 static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x0, const CUtensorMap& map_x1, const unsigned char* w_scales,
                       const QfRows& rows, const float* bias, const float* residual, TC* C, int M, int N, int kb_all, long long ldc,
                       long long ldr, int act, int* status, int splits, int stages, size_t smem, cudaStream_t s) {
-    auto kernel = q4_few_rows_kernel<NB, PIECES, TC>;
+    auto kernel = q4_few_rows_kernel<NB, MODE, TC>;
     static bool raised = false;
     if (!raised) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024) != cudaSuccess) return MU_ERR_LAUNCH;
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        cudaGetLastError();
         raised = true;
     }
     const int tiles = (N + QF_BN - 1) / QF_BN;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * splits));
-    cfg.blockDim = dim3(QF_THREADS);
+    cfg.blockDim = dim3(MODE == QF_SIXTEEN ? QF_THREADS_CUT : QF_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -310,34 +427,6 @@ static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x0, const
                               status, splits, stages) == cudaSuccess ? MU_OK : MU_ERR_LAUNCH;
 }
 
-// Whether clusters of 16 blocks of this kernel can be scheduled here (asked once).
-static int few_max_cluster() {
-    static int limit = 0;
-    if (limit == 0) {
-        int found = 8;
-        auto kernel = q4_few_rows_kernel<64, 2, float>;
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024) == cudaSuccess &&
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess) {
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(16);
-            cfg.blockDim = dim3(QF_THREADS);
-            cfg.dynamicSmemBytes = 108 * 1024;
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = 16;
-            attr[0].val.clusterDim.y = 1;
-            attr[0].val.clusterDim.z = 1;
-            cfg.attrs = attr;
-            cfg.numAttrs = 1;
-            int clusters = 0;
-            if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0) found = 16;
-        }
-        cudaGetLastError();
-        limit = found;
-    }
-    return limit;
-}
-
 static bool tensor_map_codes(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, int kp, long long row_bytes,
                              int box_rows) {
     static EncodeTiledFn fn = encode_tiled_fn();
@@ -349,6 +438,17 @@ static bool tensor_map_codes(CUtensorMap* map, CUtensorMapDataType type, const v
     return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+bool tensor_map_boxes(CUtensorMap* map, const void* base, long long rows, int cols, long long ld, int is_bf16) {
+    static EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * (is_bf16 ? 2 : 4)};
+    const cuuint32_t box[2] = {32, 32};
+    const cuuint32_t elem[2] = {1, 1};
+    return fn(map, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(base), dims, strides, box,
+              elem, CU_TENSOR_MAP_INTERLEAVE_NONE, is_bf16 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 bool tensor_map_q4(CUtensorMap* map, const void* base, long long rows, int kp, int box_rows) {
     return tensor_map_codes(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, base, rows, kp, kp / 2, box_rows);
 }
@@ -356,64 +456,72 @@ bool tensor_map_q8(CUtensorMap* map, const void* base, long long rows, int kp, i
     return tensor_map_codes(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, kp, kp, box_rows);
 }
 
-}  // namespace mu
+// How many blocks share a tile, in units of a stage (0.2 us of an SM when all take in weights).  The exchange of parts costs
+// five stages, one more for every block that takes part and one for 8 rows; a second block on an SM halves both rings.
+// Microseconds on a B200, 8-bit rows: 1 x 6,400 x 1,600 uncut 4.3, by 2 4.5, by 4 4.8; 8 x 1,600 x 6,400 uncut 13.9, by 2 8.2, by
+// 5 5.3, by 8 5.8; 8 x 4,096 x 2,048 uncut 5.3, by 2 4.5, by 4 4.6; 48 x 11,264 x 2,048 uncut 8.7, by 2 10.2, by 4 13.9.
+static int choose_splits(long long tiles, int kb_all, int rows, int sms) {
+    int best = 1;
+    long long least = 1ll << 60;
+    for (int s = 1; s <= QF_MAX_SPLIT && s <= kb_all; ++s) {
+        const long long per_sm = (tiles * s + sms - 1) / sms;                 // blocks that an SM runs, at once or in turn
+        const long long cost = per_sm * ((kb_all + s - 1) / s) + (per_sm > 1 ? 3 : 0) + (s > 1 ? 5 + s + rows / 8 : 0);
+        if (cost < least) { least = cost; best = s; }
+    }
+    return best;
+}
 
-// X: codes [M, kp] and exponents of one piece, or of two (x1 and its exponents not null); W: codes [N, kp / 2], exponents.
-// kp a multiple of 128, codes 32-byte (W) and 16-byte (X) aligned, exponents 16-byte aligned.  C bfloat16 or float32 (ldc);
-// residual float32 (ldr), may be C itself.  splits: blocks that share a tile and cut K (a power of two up to 16; 0: chosen
-// here).  `status` as mu_gemm_tc.
-MU_EXPORT int mu_q4_few_rows(const void* x0, const void* x0_scales, const void* x1, const void* x1_scales, const void* w,
-                             const void* w_scales, const float* bias, const float* residual, void* C, int M, int N, int kp,
-                             long long ldc, long long ldr, int act, int out_bf16, int splits, int* status, void* stream) {
-    if (M <= 0 || N <= 0) return MU_OK;
-    if (M > 128) return MU_ERR_UNSUPPORTED_SIZE;
-    if (kp <= 0 || kp % 128 || !x0 || !x0_scales || !w || !w_scales || !C || !status || (x1 != nullptr) != (x1_scales != nullptr))
-        return MU_ERR_BAD_ARGUMENT;
-    if (((uintptr_t)w & 31) || (((uintptr_t)x0 | (uintptr_t)x1 | (uintptr_t)x0_scales | (uintptr_t)x1_scales | (uintptr_t)w_scales) & 15))
-        return MU_ERR_ALIGNMENT;
-    if ((M > 1 && ldc < N) || (residual && M > 1 && ldr < N)) return MU_ERR_BAD_ARGUMENT;
-    if (splits < 0 || splits > mu::QF_MAX_SPLIT || (splits & (splits - 1))) return MU_ERR_BAD_ARGUMENT;
-    const int sms = mu::sm_count();
+// W: codes [N, kp / 2] and exponents; kp a multiple of 128 (pointers and strides as mu_linear_q4 has checked them).  The rows: codes x0 [M, kp] with their exponents; or two pieces, x1
+// and its exponents the second; or (x0_scales null, x1 null) bfloat16 x0 [M, K] (ldx) with K > kp - 128, M <= 16.  Codes and
+// exponents 16-byte aligned, W's codes 32-byte.  C bfloat16 or float32 (ldc); residual float32 (ldr), may be C itself.
+// splits: blocks that share a tile and cut K (up to 8; 0: chosen here).  `status` as mu_gemm_tc.
+int launch_q4_few_rows(const void* x0, const void* x0_scales, const void* x1, const void* x1_scales, long long ldx, int K,
+                             const void* w, const void* w_scales, const float* bias, const float* residual, void* C, int M, int N,
+                             int kp, long long ldc, long long ldr, int act, int out_bf16, int splits, int* status, void* stream) {
+    const int mode = !x0_scales ? QF_SIXTEEN : x1 ? QF_PIECES : QF_EIGHT;
+    if (M > (mode == QF_SIXTEEN ? QF_MAX_CUT : 64)) return MU_ERR_UNSUPPORTED_SIZE;
+    if (splits < 0 || splits > QF_MAX_SPLIT) return MU_ERR_BAD_ARGUMENT;
+    const int sms = sm_count();
     if (sms <= 0) return MU_ERR_LAUNCH;
     const long long tiles = ((long long)N + 127) / 128;
-    const int kb_all = kp / 128, pieces = x1 ? 2 : 1;
-    if (tiles * mu::QF_MAX_SPLIT > 2147483647ll) return MU_ERR_UNSUPPORTED_SIZE;
-    const int limit = mu::few_max_cluster();
-    if (splits == 0) {
-        splits = 1;
-        while (splits * 2 <= limit && tiles * splits * 2 <= sms + sms / 3 && splits * 2 <= kb_all) splits *= 2;
-    }
-    while (splits > limit || splits > kb_all) splits /= 2;
-    const int nb = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-    const size_t stage_bytes = mu::QF_W_BYTES + (size_t)pieces * nb * 128 + (1 + pieces) * 512;
-    const size_t tile_bytes = splits > 1 ? (size_t)((M + 3) / 4 * 4 + 4) * 128 * 4 : 0;
-    const int per_block = (kb_all + splits - 1) / splits;
-    size_t room = 108 * 1024;                                     // two blocks an SM where that leaves a ring of three or so
-    if (1024 + tile_bytes + 3 * stage_bytes > room) room = 220 * 1024;
-    int stages = (int)((room - 1024 - tile_bytes) / stage_bytes);
-    const int least = (int)((tile_bytes + mu::QF_W_BYTES + (size_t)pieces * nb * 128 - 1) / (mu::QF_W_BYTES + (size_t)pieces * nb * 128));
+    const int kb_all = kp / 128, pieces = mode == QF_EIGHT ? 1 : 2;
+    if (tiles * QF_MAX_SPLIT > 2147483647ll) return MU_ERR_UNSUPPORTED_SIZE;
+    if (splits == 0) splits = choose_splits(tiles, kb_all, M, sms);
+    if (splits > kb_all) splits = kb_all;
+    const int nb = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    const size_t operands = QF_W_BYTES + (size_t)pieces * nb * 128, stage_bytes = operands + (1 + pieces) * 512;
+    // the ring: half of an SM's room where there are blocks for two on one and it leaves each three stages; at least what the
+    // partial tiles take
+    const size_t parts_bytes = splits > 1 ? (size_t)((M + 3) / 4 * 4 + 4) * 4 * (128 + splits * (128 / splits + 1)) : 0;
+    const int per_block = (kb_all + splits - 1) / splits, least = (int)((parts_bytes + operands - 1) / operands);
+    const size_t room = 1024 + 3 * stage_bytes <= 111 * 1024 && tiles * splits > sms ? 111 * 1024 : 220 * 1024;
+    int stages = (int)((room - 1024) / stage_bytes);
     if (stages > per_block) stages = per_block;
-    if (stages < least) stages = least;                           // the partial tile lies on the stages
+    if (stages < least) stages = least;
     if (stages > 16) stages = 16;
     if (stages < 1) stages = 1;
-    const size_t smem = 1024 + (size_t)stages * stage_bytes + tile_bytes;
-    if (smem > 224 * 1024) return MU_ERR_UNSUPPORTED_SIZE;
-    CUtensorMap map_w, map_x0, map_x1;
-    if (!mu::tensor_map_q4(&map_w, w, N, kp, 128) || !mu::tensor_map_q8(&map_x0, x0, M, kp, nb) ||
-        !mu::tensor_map_q8(&map_x1, x1 ? x1 : x0, M, kp, nb))
-        return MU_ERR_LAUNCH;
-    const mu::QfRows rows = {{(const unsigned char*)x0_scales, (const unsigned char*)x1_scales}};
+    const size_t smem = 1024 + (size_t)stages * stage_bytes;
+    if (smem > 224 * 1024 || parts_bytes > (size_t)stages * operands || (mode == QF_SIXTEEN && stages < 4 && stages < per_block))
+        return MU_ERR_UNSUPPORTED_SIZE;
+    CUtensorMap map_w, map_x0 = {}, map_x1 = {};
+    if (!tensor_map_q4(&map_w, w, N, kp, 128)) return MU_ERR_LAUNCH;
+    if (mode != QF_SIXTEEN && !tensor_map_q8(&map_x0, x0, M, kp, nb)) return MU_ERR_LAUNCH;
+    if (mode == QF_PIECES && !tensor_map_q8(&map_x1, x1, M, kp, nb)) return MU_ERR_LAUNCH;
+    const QfRows rows = {{(const unsigned char*)x0_scales, (const unsigned char*)x1_scales}, (const __nv_bfloat16*)x0, ldx, K,
+                             K % 8 == 0 && ((uintptr_t)x0 & 15) == 0 && (M == 1 || ldx % 8 == 0)};
     cudaStream_t s = (cudaStream_t)stream;
-#define MU_FEW(NB, PIECES)                                                                                                          \
-    (out_bf16 ? mu::launch_few<NB, PIECES, __nv_bfloat16>(map_w, map_x0, map_x1, (const unsigned char*)w_scales, rows, bias, residual, \
-                                                          (__nv_bfloat16*)C, M, N, kb_all, ldc, ldr, act, status, splits, stages, smem, s) \
-              : mu::launch_few<NB, PIECES, float>(map_w, map_x0, map_x1, (const unsigned char*)w_scales, rows, bias, residual, (float*)C, \
-                                                  M, N, kb_all, ldc, ldr, act, status, splits, stages, smem, s))
-#define MU_FEW_BOTH(NB) (pieces == 2 ? MU_FEW(NB, 2) : MU_FEW(NB, 1))
+#define MU_FEW(NB, MODE)                                                                                                            \
+    (out_bf16 ? launch_few<NB, MODE, __nv_bfloat16>(map_w, map_x0, map_x1, (const unsigned char*)w_scales, rows, bias, residual, \
+                                                        (__nv_bfloat16*)C, M, N, kb_all, ldc, ldr, act, status, splits, stages, smem, s) \
+              : launch_few<NB, MODE, float>(map_w, map_x0, map_x1, (const unsigned char*)w_scales, rows, bias, residual, (float*)C, \
+                                                M, N, kb_all, ldc, ldr, act, status, splits, stages, smem, s))
+#define MU_FEW_BOTH(NB) (mode == QF_PIECES ? MU_FEW(NB, QF_PIECES) : MU_FEW(NB, QF_EIGHT))
+    if (mode == QF_SIXTEEN) return MU_FEW(16, QF_SIXTEEN);
     if (nb == 16) return MU_FEW_BOTH(16);
     if (nb == 32) return MU_FEW_BOTH(32);
-    if (nb == 64) return MU_FEW_BOTH(64);
-    return MU_FEW_BOTH(128);
+    return MU_FEW_BOTH(64);
 #undef MU_FEW_BOTH
 #undef MU_FEW
 }
+
+}  // namespace mu

@@ -1,0 +1,75 @@
+// The product with 4-bit weights as the library offers it: which of its kernels runs.
+#include "block_scaled.cuh"
+
+namespace mu {
+
+int launch_q4_few_rows(const void* x0, const void* x0_scales, const void* x1, const void* x1_scales, long long ldx, int K,
+                       const void* w, const void* w_scales, const float* bias, const float* residual, void* C, int M, int N,
+                       int kp, long long ldc, long long ldr, int act, int out_bf16, int splits, int* status, void* stream);
+int launch_q4_prompt(const void* x0, const void* x0_scales, const void* x1, const void* x1_scales, const void* w, const void* w_scales,
+                     const float* bias, const float* residual, void* C, int M, int N, int kp, long long ldc, long long ldr, int act,
+                     int out_bf16, int bn, int* status, void* stream);
+int launch_quantize_q8(const void* x, long long ldx, int is_bf16, int m, int k, int kp, int pieces, void* codes, void* scales, void* stream);
+
+// Up to 32 rows go to the kernel with the weights as the wide operand; up to 64 where that kernel can cut a long k and the other
+// would leave most SMs idle.  Microseconds, 8-bit rows, that kernel and the other: 8 x 6,400 x 1,600 4.5 and 6.3; 32 x 11,264 x
+// 2,048 7.2 and 9.4; 32 x 6,400 x 1,600 6.1 and 5.8; 64 x 1,600 x 6,400 8.4 and 12.3; 64 x 4,096 x 2,048 9.0 and 5.9.
+static bool few_rows(int m, int n, int kp, int sms) {
+    return m <= 32 || (m <= 64 && kp >= 32 * 128 && ((long long)n + 127) / 128 * 4 <= sms);
+}
+
+}  // namespace mu
+
+// The arguments come as one packed record: a call with twenty of them costs the caller's side more than the launch.
+struct LinearQ4Args {
+    const void *x, *x_scales;            // 8-bit rows: codes [m, kp] and exponents; bfloat16 rows [m, k] (ldx): exponents null
+    const void *w, *w_scales;            // codes [n, kp / 2], exponents
+    const float *bias, *residual;        // null or [n]; null or [m, n] (ldr), may be out
+    void *out, *room;                    // out [m, n] (ldo); room for the pieces of more than 16 bfloat16 rows (mu_linear_q4_room)
+    int* status;
+    void* stream;
+    long long ldx, ldo, ldr;
+    int m, n, k, kp, act, out_bf16, way; // way 0: the kernel is chosen here; tests: 1 + blocks a tile, or -(columns of a tile)
+    int unused;
+};
+
+constexpr int Q4_CUT_INSIDE = 16;        // bfloat16 rows that the few-rows kernel cuts itself
+
+// Room for the pieces of bfloat16 rows: both pieces' codes, then both pieces' exponents.
+MU_EXPORT long long mu_linear_q4_room(int m, int kp) {
+    return m <= Q4_CUT_INSIDE ? 0 : 2ll * m * kp + 2ll * ((m + 127) / 128) * 128 * (kp / 32);
+}
+MU_EXPORT int mu_linear_q4_args_size() { return (int)sizeof(LinearQ4Args); }
+
+MU_EXPORT int mu_linear_q4(const LinearQ4Args* p) {
+    const LinearQ4Args a = *p;
+    if (a.m <= 0 || a.n <= 0) return MU_OK;
+    const bool sixteen = !a.x_scales;
+    if (a.kp <= 0 || a.kp % 128 || a.k <= a.kp - 128 || a.k > a.kp || !a.x || !a.w || !a.w_scales || !a.out || !a.status) return MU_ERR_BAD_ARGUMENT;
+    // (one row's stride is never used)
+    if (a.m > 1 && (a.ldo < a.n || (a.residual && a.ldr < a.n) || (sixteen && a.ldx < a.k))) return MU_ERR_BAD_ARGUMENT;
+    if (((uintptr_t)a.w & 31) || (((uintptr_t)a.w_scales | (uintptr_t)a.x_scales | (uintptr_t)a.room) & 15) || ((uintptr_t)a.x & (sixteen ? 1 : 15)) ||
+        ((uintptr_t)a.out & (a.out_bf16 ? 1 : 3)))
+        return MU_ERR_ALIGNMENT;
+    const int sms = mu::sm_count();
+    if (sms <= 0) return MU_ERR_LAUNCH;
+    const long long ldo = a.m > 1 ? a.ldo : a.n, ldr = a.m > 1 ? a.ldr : a.n, ldx = a.m > 1 ? a.ldx : a.k;
+    const void *x0 = a.x, *s0 = a.x_scales, *x1 = nullptr, *s1 = nullptr;
+    const bool few = a.way > 0 || (a.way == 0 && mu::few_rows(a.m, a.n, a.kp, sms));
+    if (sixteen && (a.m > Q4_CUT_INSIDE || !few)) {
+        if (!a.room) return MU_ERR_BAD_ARGUMENT;
+        const long long codes = (long long)a.m * a.kp, scales = ((long long)a.m + 127) / 128 * 128 * (a.kp / 32);
+        unsigned char* r = (unsigned char*)a.room;
+        const int code = mu::launch_quantize_q8(a.x, ldx, 1, a.m, a.k, a.kp, 2, r, r + 2 * codes, a.stream);
+        if (code != MU_OK) return code;
+        x0 = r;
+        x1 = r + codes;
+        s0 = r + 2 * codes;
+        s1 = r + 2 * codes + scales;
+    }
+    if (few)
+        return mu::launch_q4_few_rows(x0, s0, x1, s1, ldx, a.k, a.w, a.w_scales, a.bias, a.residual, a.out, a.m, a.n, a.kp, ldo, ldr, a.act,
+                                      a.out_bf16, a.way > 0 ? a.way - 1 : 0, a.status, a.stream);
+    return mu::launch_q4_prompt(x0, s0, x1, s1, a.w, a.w_scales, a.bias, a.residual, a.out, a.m, a.n, a.kp, ldo, ldr, a.act, a.out_bf16, -a.way,
+                                a.status, a.stream);
+}

@@ -12,17 +12,19 @@
 
 namespace mu {
 
-__device__ __forceinline__ float group_max(float top) {           // over the four lanes that hold a group, eight entries each
+__device__ __forceinline__ unsigned int group_max(unsigned int top) {      // over the four lanes that hold a group, eight entries each
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    return max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+}
+__device__ __forceinline__ unsigned int max_of_eight(const float (&v)[8]) {
+    unsigned int top = 0;
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) top = larger_magnitude(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int i = 0; i < 8; ++i) top = max(top, magnitude_bits(v[i]));
     return top;
 }
-__device__ __forceinline__ float max_of_eight(const float (&v)[8]) {
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = larger_magnitude(top, v[i]);
-    return top;
-}
+
+// Two bfloat16 that were widened, as they lay in memory.
+__device__ __forceinline__ unsigned int bf16_words(float lo, float hi) { return __float_as_uint(lo) >> 16 | (__float_as_uint(hi) & 0xFFFF0000u); }
 
 // Eight entries of a row from column c on; columns from k on are zeros.
 template <bool VEC, typename TE>
@@ -82,16 +84,16 @@ quantize_q4_kernel(const TE* __restrict__ w, long long ldw, int n, int k, int kp
         return;
     }
     float v[32];
-    float top = 0.0f;
+    unsigned int top = 0;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
         const int c = g * BS_GROUP + i;
         v[i] = c < k ? to_float(w[row * ldw + c]) : 0.0f;
-        top = larger_magnitude(top, v[i]);
+        top = max(top, magnitude_bits(v[i]));
     }
     uint4 packed = make_uint4(0, 0, 0, 0);
     int b = 255;                                                   // a group holding an infinity or NaN is NaN
-    if (is_finite_magnitude(top)) {
+    if (is_number(top)) {
         b = exponent_e2m1(top);
         if (b > 0 && e2m1_error(v, b - 1) < e2m1_error(v, b)) --b;
         const float f = inverse_scale(b);
@@ -103,44 +105,65 @@ quantize_q4_kernel(const TE* __restrict__ w, long long ldw, int n, int k, int kp
     }
     *reinterpret_cast<uint4*>(codes + row * (kp / 2) + (long long)g * 16) = packed;
     *at = (unsigned char)b;
+    // a product launched next may fetch its weights before it waits for this kernel's end: what is written is in memory by
+    // the time this block has gone
+    __threadfence();
+    asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
 // ------------------------------------------------------------------------------------------------- rows
-// Eight entries a thread, four neighbouring lanes a group.  PIECES = 2: the second piece's codes lie `rows x kp` bytes, its
-// exponents a whole set of tiles, behind the first's.
-template <typename TE, int PIECES, bool VEC>
+// Eight entries a thread, four neighbouring lanes a group, ROWS rows a thread, all asked for before any is worked on: one where
+// that makes no more blocks than the SMs hold at a time, four for more.
+// PIECES = 2: the second piece's codes lie `m x kp` bytes, its exponents a whole set of tiles, behind the first's.
+template <typename TE, int PIECES, bool VEC, int ROWS>
 __global__ void __launch_bounds__(256)
 quantize_q8_kernel(const TE* __restrict__ x, long long ldx, int m, int k, int kp, unsigned char* __restrict__ codes,
                    unsigned char* __restrict__ scales) {
     pdl_trigger();
     pdl_wait();
-    const int eights = kp / 8;
-    const long long item = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const long long row = item / eights;
-    const int c = (int)(item % eights) * 8;
-    const long long rows = ((long long)m + BS_TILE - 1) / BS_TILE * BS_TILE;
-    const bool real = row < m;
-    float v[8];
-    if (real) load_eight<VEC>(x + row * ldx, c, k, v);
-    else {
+    const int row0 = blockIdx.x * blockDim.y * ROWS + threadIdx.y, c = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
+    const int rows = (m + BS_TILE - 1) / BS_TILE * BS_TILE;
+    float v[ROWS][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    for (int j = 0; j < ROWS; ++j) {
+        const int row = row0 + j * blockDim.y;
+        if (row < m && c < kp) load_eight<VEC>(x + (long long)row * ldx, c, k, v[j]);
+        else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[j][i] = 0.0f;
+        }
     }
-    const float top = group_max(max_of_eight(v));                  // (every lane of the warp takes part)
-    const bool fine = is_finite_magnitude(top);
-    const int b = fine ? exponent_e4m3(top) : 127;
-    if (real) {
-        uint2 hi, lo;
-        if (PIECES == 2) e4m3_pieces_of_eight(v, b, hi, lo);
-        else hi = e4m3_of_eight(v, b);
-        if (!fine) hi = lo = make_uint2(E4M3_NAN4, E4M3_NAN4);
-        *reinterpret_cast<uint2*>(codes + row * kp + c) = hi;
-        if (PIECES == 2) *reinterpret_cast<uint2*>(codes + ((long long)m + row) * kp + c) = lo;
-    }
-    if (row < rows && c % BS_GROUP == 0) {
-        unsigned char* at = scales + scale_at(row, c / BS_GROUP, kp / BS_TILE);
-        *at = (unsigned char)b;
-        if (PIECES == 2) at[rows * (kp / BS_GROUP)] = (unsigned char)low_exponent(b);
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+        const int row = row0 + j * blockDim.y;
+        const unsigned int top = group_max(max_of_eight(v[j]));    // (every lane of the warp takes part)
+        const bool fine = is_number(top);
+        const int b = fine ? exponent_e4m3(top) : 127;
+        if (row < m && c < kp) {
+            uint2 hi, lo;
+            if (PIECES == 2) {
+                const unsigned int words[4] = {bf16_words(v[j][0], v[j][1]), bf16_words(v[j][2], v[j][3]), bf16_words(v[j][4], v[j][5]),
+                                               bf16_words(v[j][6], v[j][7])};
+                e4m3_pieces_of_eight(words, b, hi, lo);
+            } else {
+                hi = e4m3_of_eight(v[j], b);
+            }
+            if (!fine) hi = lo = make_uint2(E4M3_NAN4, E4M3_NAN4);
+            *reinterpret_cast<uint2*>(codes + (long long)row * kp + c) = hi;
+            if (PIECES == 2) *reinterpret_cast<uint2*>(codes + ((long long)m + row) * kp + c) = lo;
+        }
+        // sixteen lanes hold 128 columns, a word of exponents
+        unsigned int word = (unsigned int)b << (8 * (c / BS_GROUP % 4));
+        word |= __shfl_xor_sync(0xffffffffu, word, 4);
+        word |= __shfl_xor_sync(0xffffffffu, word, 8);
+        if (row < rows && c < kp && c % BS_TILE == 0) {
+            unsigned int low = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) low |= (unsigned int)low_exponent(word >> (8 * i) & 255u) << (8 * i);
+            unsigned char* at = scales + scale_at(row, c / BS_GROUP, kp / BS_TILE);
+            *reinterpret_cast<unsigned int*>(at) = word;
+            if (PIECES == 2) *reinterpret_cast<unsigned int*>(at + (long long)rows * (kp / BS_GROUP)) = low;
+        }
     }
 }
 
@@ -193,8 +216,8 @@ residual_add_norm_q8_kernel(float* __restrict__ x, long long ldx, const Addend a
         load_eight<VEC>(weight, c, width, g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * g[i];
-        const float top = group_max(max_of_eight(v));
-        const bool fine = is_finite_magnitude(top);
+        const unsigned int top = group_max(max_of_eight(v));
+        const bool fine = is_number(top);
         const int b = fine ? exponent_e4m3(top) : 127;
         const uint2 code = fine ? e4m3_of_eight(v, b) : make_uint2(E4M3_NAN4, E4M3_NAN4);
         if (c < kp) {
@@ -238,39 +261,66 @@ MU_EXPORT int mu_quantize_q4(const void* w, long long ldw, int is_bf16, int n, i
     return MU_OK;
 }
 
+namespace mu {
+
 // x [m, k] (ldx) bfloat16 or float32 -> codes [pieces, m, kp], scales [pieces, ceil(m / 128), kp / 128, 512].
-MU_EXPORT int mu_quantize_q8(const void* x, long long ldx, int is_bf16, int m, int k, int kp, int pieces, void* codes,
-                             void* scales, void* stream) {
-    if (m <= 0) return MU_OK;
-    if (!x || !codes || !scales || k <= 0 || kp % 128 || kp < k || kp - k >= 128 || (m > 1 && ldx < k) || pieces < 1 || pieces > 2 ||
-        (pieces == 2 && !is_bf16))
-        return MU_ERR_BAD_ARGUMENT;
-    if (((uintptr_t)codes | (uintptr_t)scales) & 15) return MU_ERR_ALIGNMENT;
-    const long long rows = ((long long)m + 127) / 128 * 128, items = rows * (kp / 8);
-    const long long blocks = (items + 255) / 256;
-    if (blocks > 2147483647ll) return MU_ERR_UNSUPPORTED_SIZE;
+int launch_quantize_q8(const void* x, long long ldx, int is_bf16, int m, int k, int kp, int pieces, void* codes, void* scales, void* stream) {
+    const int rows = (m + 127) / 128 * 128, eights = kp / 8;
+    // a block's threads along a row and its rows: whole warps of a row where it has as many eights
+    const int along = eights >= 256 ? 256 : eights >= 128 ? 128 : eights >= 64 ? 64 : eights >= 32 ? 32 : 16;
+    const int deep = 256 / along;
+    const bool many = rows * (long long)eights >= 2ll * 148 * 2048;
+    const int each = many ? 4 : 1;
+    const dim3 block(along, deep), grid((unsigned)((rows + deep * each - 1) / (deep * each)), (eights + along - 1) / along);
+    if (grid.y > 65535) return MU_ERR_UNSUPPORTED_SIZE;
     const bool vec = k % 8 == 0 && ((uintptr_t)x & 15) == 0 && (m == 1 || ldx % (is_bf16 ? 8 : 4) == 0);
     cudaStream_t s = (cudaStream_t)stream;
-#define MU_Q8(TE, PIECES, VEC) \
-    return mu::launch_pdl(mu::quantize_q8_kernel<TE, PIECES, VEC>, dim3((unsigned)blocks), dim3(256), 0, s, 1, (const TE*)x, ldx, m, k, kp, \
-                          (unsigned char*)codes, (unsigned char*)scales)
-    if (pieces == 2) { if (vec) MU_Q8(__nv_bfloat16, 2, true); MU_Q8(__nv_bfloat16, 2, false); }
-    if (is_bf16) { if (vec) MU_Q8(__nv_bfloat16, 1, true); MU_Q8(__nv_bfloat16, 1, false); }
-    if (vec) MU_Q8(float, 1, true);
-    MU_Q8(float, 1, false);
+#define MU_Q8_ROWS(TE, PIECES, VEC, ROWS) \
+    return launch_pdl(quantize_q8_kernel<TE, PIECES, VEC, ROWS>, grid, block, 0, s, 1, (const TE*)x, ldx, m, k, kp, (unsigned char*)codes, (unsigned char*)scales)
+#define MU_Q8(TE, PIECES, VEC) { if (many) MU_Q8_ROWS(TE, PIECES, VEC, 4); MU_Q8_ROWS(TE, PIECES, VEC, 1); }
+    if (pieces == 2) { if (vec) MU_Q8(__nv_bfloat16, 2, true) MU_Q8(__nv_bfloat16, 2, false) }
+    if (is_bf16) { if (vec) MU_Q8(__nv_bfloat16, 1, true) MU_Q8(__nv_bfloat16, 1, false) }
+    if (vec) MU_Q8(float, 1, true)
+    MU_Q8(float, 1, false)
+#undef MU_Q8_ROWS
 #undef MU_Q8
 }
 
-// As mu_residual_add_norm with one group, the normed rows in 8 bits: codes [m, kp], scales [ceil(m / 128), kp / 128, 512].
-MU_EXPORT int mu_residual_add_norm_q8(float* x, long long ldx, const float* y, long long ldy, float mult, const float* y2,
-                                      long long ldy2, float mult2, const float* scale, const float* weight, float eps, int m,
-                                      int width, int kp, void* codes, void* scales, void* stream) {
+}  // namespace mu
+
+MU_EXPORT int mu_quantize_q8(const void* x, long long ldx, int is_bf16, int m, int k, int kp, void* codes, void* scales, void* stream) {
+    if (m <= 0) return MU_OK;
+    if (!x || !codes || !scales || k <= 0 || kp % 128 || kp < k || kp - k >= 128 || (m > 1 && ldx < k)) return MU_ERR_BAD_ARGUMENT;
+    if (((uintptr_t)codes | (uintptr_t)scales) & 15) return MU_ERR_ALIGNMENT;
+    return mu::launch_quantize_q8(x, m > 1 ? ldx : k, is_bf16, m, k, kp, 1, codes, scales, stream);
+}
+
+// As mu_residual_add_norm with one group, the normed rows in 8 bits: codes [m, kp], scales [ceil(m / 128), kp / 128, 512].  The
+// arguments come as one packed record (q4_linear.cu says why).
+struct NormQ8Args {
+    float* x;
+    const float *y, *y2, *scale, *weight;
+    void *codes, *scales, *stream;
+    long long ldx, ldy, ldy2;
+    float mult, mult2, eps;
+    int m, width, kp;
+};
+MU_EXPORT int mu_norm_q8_args_size() { return (int)sizeof(NormQ8Args); }
+
+MU_EXPORT int mu_residual_add_norm_q8(const NormQ8Args* p) {
+    const NormQ8Args a = *p;
+    float* x = a.x;
+    const float *y = a.y, *y2 = a.y2, *scale = a.scale, *weight = a.weight;
+    const long long ldx = a.ldx, ldy = a.ldy, ldy2 = a.ldy2;
+    const float mult = a.mult, mult2 = a.mult2, eps = a.eps;
+    const int m = a.m, width = a.width, kp = a.kp;
+    void *codes = a.codes, *scales = a.scales, *stream = a.stream;
     if (m <= 0) return MU_OK;
     if (!x || !weight || !codes || !scales || width <= 0 || kp % 128 || kp < width || kp - width >= 128 || (y2 && !y) || (scale && !y))
         return MU_ERR_BAD_ARGUMENT;
     if (((uintptr_t)codes | (uintptr_t)scales) & 15) return MU_ERR_ALIGNMENT;
     const mu::Addend add = {y, ldy, mult, y2, ldy2, mult2, scale};
-    const bool vec = width % 8 == 0 && ldx % 4 == 0 && ldy % 4 == 0 && ldy2 % 4 == 0 &&
+    const bool vec = width % 8 == 0 && (m == 1 || (ldx % 4 == 0 && ldy % 4 == 0 && ldy2 % 4 == 0)) &&
                      (((uintptr_t)x | (uintptr_t)y | (uintptr_t)y2 | (uintptr_t)scale | (uintptr_t)weight) & 15) == 0;
     cudaStream_t s = (cudaStream_t)stream;
 #define MU_NORM8(THREADS, KEEP, VEC)                                                                                            \

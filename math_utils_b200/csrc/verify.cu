@@ -431,18 +431,33 @@ verify_walk_kernel(const VerifyRows rows, const VerifyPart* __restrict__ parts_o
 
 }  // namespace mu
 
-// Bytes of scratch for a call: 24 a part of a row.
-MU_EXPORT int mu_verify_scratch(int batch, int drafts, int parts) {
-    const long long n = (long long)batch * (2ll * drafts + 1) * parts * (long long)sizeof(mu::VerifyPart);
-    return n > 2147483647ll ? -1 : (int)n;
-}
-
 // target [batch, drafts + 1, vocab] and draft [batch, drafts, vocab] float32 (strides of sequences and rows in elements;
-// draft may be null where greedy); draft_tokens [batch, drafts] int32; draws [batch, drafts + 1] float64; top_k 0: all.
-// tokens [batch, drafts + 1] (the drafts taken, the token after them, then -1) and kept [batch] int32.
-MU_EXPORT int mu_verify_drafts(const float* target, long long target_seq, long long target_row, const float* draft, long long draft_seq,
-                               long long draft_row, int batch, int drafts, int vocab, const int* draft_tokens, const double* draws,
-                               double temperature, int top_k, int parts, void* scratch, int* tokens, int* kept, void* stream) {
+// draft may be null where greedy); draft_tokens [batch, drafts] int32; draws [batch, drafts + 1] float64; top_k 0: all; room: 24
+// bytes for each of `parts` parts of every row read.  tokens [batch, drafts + 1] (the drafts taken, the token after them,
+// then -1) and kept [batch] int32.  One packed record (q4_linear.cu says why).
+struct VerifyArgs {
+    const float *target, *draft;
+    const int* draft_tokens;
+    const double* draws;
+    void* room;
+    int *tokens, *kept;
+    void* stream;
+    long long target_seq, target_row, draft_seq, draft_row;
+    double temperature;
+    int batch, drafts, vocab, top_k, parts, unused;
+};
+static_assert(sizeof(mu::VerifyPart) == 24, "what the caller gives room for");
+MU_EXPORT int mu_verify_args_size() { return (int)sizeof(VerifyArgs); }
+
+MU_EXPORT int mu_verify_drafts(const VerifyArgs* record) {
+    const VerifyArgs a = *record;
+    const float *target = a.target, *draft = a.draft;
+    const int* draft_tokens = a.draft_tokens;
+    const double* draws = a.draws;
+    void *scratch = a.room, *stream = a.stream;
+    int *tokens = a.tokens, *kept = a.kept, parts = a.parts;
+    const int batch = a.batch, drafts = a.drafts, vocab = a.vocab, top_k = a.top_k;
+    const double temperature = a.temperature;
     if (batch <= 0) return MU_OK;
     const bool greedy = !(temperature > 0.0) || top_k == 1;
     if (!target || drafts < 0 || vocab <= 0 || (drafts > 0 && !draft_tokens) || !draws || !scratch || !tokens || !kept || top_k < 0 ||
@@ -451,7 +466,7 @@ MU_EXPORT int mu_verify_drafts(const float* target, long long target_seq, long l
     const long long n_rows = (long long)batch * (drafts + 1) + (greedy ? 0 : (long long)batch * drafts);
     if (n_rows > 2147483647ll || (long long)batch * mu::VW_BLOCKS > 2147483647ll) return MU_ERR_UNSUPPORTED_SIZE;
     if ((uintptr_t)scratch & 7) return MU_ERR_ALIGNMENT;
-    const mu::VerifyRows rows = {target, draft, target_seq, target_row, draft_seq, draft_row, batch, drafts, vocab};
+    const mu::VerifyRows rows = {target, draft, a.target_seq, a.target_row, a.draft_seq, a.draft_row, batch, drafts, vocab};
     cudaStream_t s = (cudaStream_t)stream;
     const bool cuts = !greedy && top_k > 0 && top_k < vocab;
     const double inv_td = greedy ? 1.0 : 1.0 / temperature;
