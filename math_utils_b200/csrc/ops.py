@@ -2007,7 +2007,7 @@ def sample(logits: torch.Tensor, temperature: float, top_k: int, seed: int,
     return out
 
 
-VERIFY_PART_BYTES = 24         # VerifyPart in verify.cu
+VERIFY_PART_BYTES, VERIFY_LIST = 32, 512         # sizeof(VerifyPart) and VERIFY_LIST in verify.cu
 
 
 def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], drafts: torch.Tensor, draws: torch.Tensor,
@@ -2045,8 +2045,9 @@ def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], dr
     if b == 0:
         return tokens, kept
     rows = b * (g + 1 if greedy else 2 * g + 1)
-    parts = max(1, min(16, 592 // rows, vocab // 4096))       # blocks a row: four an SM where the row is long enough
-    room = _new(logits, torch.uint8, rows * parts * VERIFY_PART_BYTES)
+    cuts = not greedy and 0 < top_k < vocab
+    parts = 1 if cuts else max(1, min(16, 2400 // rows, vocab // 4096))       # blocks a row: sixteen an SM where the row is long enough
+    room = _new(logits, torch.uint8, rows * (parts * VERIFY_PART_BYTES + (8 * top_k if cuts and top_k <= VERIFY_LIST else 0)))
     q = draft_logits if g > 0 and not greedy else None
     _check(library().mu_verify_drafts(_VERIFY_ARGS.pack(
         logits.data_ptr(), 0 if q is None else q.data_ptr(), drafts.data_ptr(), draws.data_ptr(), room.data_ptr(), tokens.data_ptr(),
