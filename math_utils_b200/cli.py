@@ -1,7 +1,8 @@
 """Command line, in the manner of the reference's ``src/LLM.cpp``.
 
     llm <model-dir> [--tokens N] [--temp F] [--topk N] [--seed N] [--ctx N]
-        [--prompt IDS] [--random] [--config FILE] [--fp32] [--stop IDS] [--profile] [--load-only]
+        [--prompt IDS] [--random] [--config FILE] [--fp32] [--q4] [--rows8] [--drafts N] [--stop IDS] [--profile]
+        [--load-only]
 
 Option names, meanings and defaults are the reference's (src/LLM.cpp:88-128,
 215-282): ``--tokens`` 256, ``--temp`` 0.7, ``--topk`` 20, ``--seed`` 0,
@@ -47,6 +48,10 @@ def build_parser() -> argparse.ArgumentParser:
                     help="run the topology of config.json with invented weights (see --config)")
     ap.add_argument("--config", help="with --random: a config.json to invent weights for")
     ap.add_argument("--fp32", action="store_true", help="the true 32-bit path instead of bfloat16")
+    ap.add_argument("--q4", action="store_true", help="the layers' matrices in 4 bits")
+    ap.add_argument("--rows8", action="store_true", help="with --q4: the rows that meet 4-bit matrices in 8 bits too")
+    ap.add_argument("--drafts", type=int, default=0,
+                    help="tokens that the model in 4 bits drafts a step, for the model itself to verify; 0 is none")
     ap.add_argument("--stop", help="stop token ids (default: eos_token_id of config.json)")
     ap.add_argument("--profile", action="store_true",
                     help="print load time and, per answer, prompt and generation rates and per-stage device times "
@@ -78,7 +83,8 @@ def main(argv=None) -> int:
     t0 = time.time()
     llm = LLM(model_dir, Options(context=args.ctx, max_tokens=args.tokens, temperature=args.temp,
                                  top_k=args.topk, seed=args.seed, dtype="float32" if args.fp32 else "bfloat16",
-                                 profile=args.profile))
+                                 profile=args.profile, weight_bits=4 if args.q4 else 16,
+                                 row_bits=8 if args.rows8 and args.q4 else 16, drafts=args.drafts))
     if args.stop is not None:
         llm.model.stop_ids = tuple(parse_ids(args.stop))
     load_s = time.time() - t0

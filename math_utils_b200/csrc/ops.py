@@ -197,6 +197,8 @@ _SIGNATURES = {
     "mu_linear_q4": [ctypes.c_char_p],
     "mu_norm_q8_args_size": [],
     "mu_linear_q4_args_size": [],
+    "mu_sample": [_c_p, _c_ll, _c_int, _c_int, _c_f, _c_int, _c_ull, _c_p, _c_p, _c_p, _c_p, _c_p, _c_int,
+                  _c_p, _c_p, _c_p],
 }
 
 
@@ -1811,6 +1813,14 @@ def quantize_q8(x: torch.Tensor) -> Q8Rows:
     _check(library().mu_quantize_q8(_ptr(x), x.stride(0), is_bf16, m, k, kp, _ptr(codes), _ptr(scales), _stream()),
            ("quantize_q8({}x{})", m, k))
     return Q8Rows(codes, scales)
+
+
+def q8_values(rows: Q8Rows) -> torch.Tensor:
+    """What rows in 8 bits stand for, float32 [m, kp]: for an onlooker (the kernels read the codes)."""
+    codes, scales = rows
+    m, kp = codes.shape
+    e = scales.view(torch.uint8).permute(0, 3, 2, 1, 4).reshape(-1, kp // 32)[:m]
+    return (codes.float().unflatten(1, (-1, 32)) * torch.exp2(e.float() - 127.0)[..., None]).flatten(1)
 
 
 def residual_add_norm_q8(x: torch.Tensor, y: Optional[torch.Tensor], mult: float, weight: torch.Tensor, eps: float,

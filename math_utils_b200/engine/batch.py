@@ -93,6 +93,8 @@ class StepContext:
             if hasattr(tensor, "materialize"):
                 # (a trace that only keeps time does not look at values: nothing is computed for it)
                 tensor = tensor.materialize_copy() if getattr(self.trace, "wants_values", True) else None
+            elif isinstance(tensor, tuple):               # rows in 8 bits: their values, columns rounded up to 128
+                tensor = self.runtime.ops.q8_values(tensor) if getattr(self.trace, "wants_values", True) else None
             self.trace(self.tag + name, tensor)
 
     def flush_join(self) -> None:

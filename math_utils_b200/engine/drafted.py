@@ -1,0 +1,198 @@
+"""Generation with drafted tokens: a draft model proposes a few tokens a step, the target verifies them in one.
+
+One round for a batch: the draft model steps ``drafts`` + 1 times from a recorded single-token step
+(``DecodeSession``), each sample feeding the next; the target then runs the tokens so far unseen (the last one kept and
+the drafts) as ONE step with the logits of every position wanted, which costs it little more than a single token does;
+``ops.verify_drafts`` says which drafts stand and what follows them, so that the tokens are distributed as the
+target's own (greedy: are the target's own).  Both caches are then cut back to what stood.
+
+Any two models over one vocabulary will do; the natural draft is the same weights in 4 bits.  Caches that cannot be cut
+back (windows, fixed-size state) are refused.  Random numbers: a request's draws depend on its seed and index alone; the
+draft's samples and the verification use streams of their own.
+"""
+from __future__ import annotations
+
+from typing import List, Optional, Sequence
+
+import numpy as np
+import torch
+
+from ..sampling import Sampler, SamplingParams
+from ..sampling.sampler import uniform_draws
+from .batch import StepEntry
+from .decode_session import session_for
+from .generate import check_kernels, settle, take_token
+
+_DRAFT_STREAM = 0x5851F42D4C957F2D         # what the draft's seed differs by
+
+
+def check_draftable(model, draft, cache, draft_cache) -> None:
+    """Raises ValueError where the two cannot work together."""
+    if model.vocab_size != draft.vocab_size:
+        raise ValueError(f"the draft has a vocabulary of {draft.vocab_size}, the model one of {model.vocab_size}")
+    for what, m, c in (("model", model, cache), ("draft", draft, draft_cache)):
+        if c.has_running_state or any(g.spec.window > 0 for g in c.kv_groups):
+            raise ValueError(f"drafted tokens need caches that can be cut back: the {what} has windows or fixed-size state")
+        if not m.graph_safe:
+            raise ValueError(f"drafted tokens need a {what} whose single-token step can be recorded")
+
+
+def room_for_drafts(model, draft, lengths: Sequence[int], drafts: int, context: int) -> int:
+    """How many tokens may be drafted in a round for sequences of these lengths (positions in the cache): the step runs
+    one token more, and no position past the context or either model's last is touched."""
+    most = min(context, model.max_positions, draft.max_positions)
+    return max(0, min([drafts] + [most - n - 1 for n in lengths]))
+
+
+def run_drafted(model, draft, cache, draft_cache, params: SamplingParams, states, stop_ids, max_tokens: int, context: int,
+                drafts: int, kept_slots: Optional[Sequence] = None, first_sample: Optional[list] = None,
+                counts: Optional[dict] = None) -> None:
+    """One batch from start to end, as ``run_batch_graphed`` but with ``drafts`` tokens drafted a round.
+    ``kept_slots``: a (slot, draft slot) pair for each request, taken by the caller; they are not given back, and at the end
+    hold exactly what was fed and emitted.  ``counts``: receives ``rounds``, ``drafted`` and ``kept``."""
+    check_draftable(model, draft, cache, draft_cache)
+    ops, device = model.runtime.ops, model.runtime.device
+    draft_params = SamplingParams(params.temperature, params.top_k, params.seed ^ _DRAFT_STREAM)
+    tally = counts if counts is not None else {}
+    tally.update(rounds=0, drafted=0, kept=0)
+    slots = {}
+    try:
+        live = []
+        for k, st in enumerate(states):
+            if max_tokens <= 0 or st.held + len(st.prompt) >= context:
+                st.finished, st.reason = True, "max_tokens" if max_tokens <= 0 else "context"
+                continue
+            slots[k] = kept_slots[k] if kept_slots is not None else (cache.acquire(), draft_cache.acquire())
+            live.append(k)
+        if not live:
+            return
+
+        def leave(k):
+            pair = slots.pop(k)
+            if kept_slots is None:
+                cache.release(pair[0])
+                draft_cache.release(pair[1])
+
+        prompts = [list(states[k].prompt) for k in live]
+        sampler = Sampler(params, [states[k].index for k in live], device, ops)
+        logits = model.step(cache, [StepEntry(slots[k][0], p, [len(p) - 1]) for k, p in zip(live, prompts)])
+        first = sampler.sample(logits)
+        draft.step(draft_cache, [StepEntry(slots[k][1], p) for k, p in zip(live, prompts)])
+        last = dict(zip(live, first.cpu().tolist()))           # the token each request has produced and not been fed
+        if first_sample is not None:
+            import time
+            first_sample.append(time.perf_counter())
+        check_kernels(model)
+        used = {k: 1 for k in live}                            # draws of each request's own stream
+        drawn = 0                                              # draws of the draft's streams, the same for all
+        for k in list(live):
+            if not take_token(states[k], last[k], stop_ids, max_tokens, context):
+                live.remove(k)
+                leave(k)
+        while live:
+            starts = [cache.length(slots[k][0]) for k in live]
+            g = room_for_drafts(model, draft, starts, drafts, context)
+            n = len(live)
+            ids, qs = _draft(draft, draft_cache, draft_params, [slots[k][1] for k in live], [states[k].index for k in live],
+                             [last[k] for k in live], g, drawn)
+            drawn += g + 1
+            rows = ids.cpu().tolist() if g else [[] for _ in live]
+            logits = model.step(cache, [StepEntry(slots[k][0], [last[k]] + r, range(g + 1)) for k, r in zip(live, rows)])
+            draws = np.stack([uniform_draws(params.seed, states[k].index, used[k], g + 1) for k in live])
+            tokens, kept = ops.verify_drafts(logits.view(n, g + 1, -1), qs, ids, torch.from_numpy(draws).to(device),
+                                             params.temperature if not params.greedy else 0.0, params.kept)
+            answer = torch.cat([tokens, kept[:, None]], dim=1).cpu().tolist()
+            check_kernels(model)
+            tally["rounds"] += 1
+            tally["drafted"] += g * n
+            for k, start, row in zip(list(live), starts, answer):
+                stood = row[-1]
+                tally["kept"] += stood
+                used[k] += g + 1
+                # what both models have been fed and what stands of it: the last token and the drafts kept
+                cache.truncate(slots[k][0], start + 1 + stood)
+                draft_cache.truncate(slots[k][1], start + 1 + stood)
+                goes_on = True
+                for i, token in enumerate(row[:stood + 1]):
+                    goes_on = take_token(states[k], token, stop_ids, max_tokens, context)
+                    if not goes_on:
+                        # what was kept behind this token has been fed, but is no part of the answer
+                        cut = start + 1 + min(i, stood)
+                        cache.truncate(slots[k][0], cut)
+                        draft_cache.truncate(slots[k][1], cut)
+                        break
+                last[k] = states[k].produced[-1] if states[k].produced else last[k]
+                if not goes_on:
+                    live.remove(k)
+                    leave(k)
+        if kept_slots is not None:
+            settle(model, cache, states, [pair[0] for pair in kept_slots], context)
+            settle(draft, draft_cache, states, [pair[1] for pair in kept_slots], context)
+    finally:
+        if kept_slots is None:
+            for a, b in slots.values():
+                cache.release(a)
+                draft_cache.release(b)
+
+
+def _draft(draft, cache, params: SamplingParams, slots: Sequence[int], requests: Sequence[int], tokens: Sequence[int], g: int,
+           drawn: int):
+    """``g`` tokens drafted behind ``tokens``: (ids int32 [n, g], the logits they were sampled from [n, g, vocab], or None
+    where greedy).  The draft is stepped once more, so that its cache holds the last one too."""
+    n, device = len(slots), draft.runtime.device
+    session = session_for(draft, cache, params, n, pipelined=False)
+    state = (list(slots), list(requests), drawn)
+    if getattr(session, "drafts_for", None) != state:          # (else it is where the round before left it)
+        session.rebind(slots, requests, [drawn] * n)
+    session.drafts_for = (list(slots), list(requests), drawn + g + 1)
+    starts = [cache.reserve(s, g + 1) for s in slots]
+    session.sync_block_tables()
+    session.feed(tokens, starts)
+    ids = torch.empty((n, g), dtype=torch.int32, device=device)
+    qs = None if params.greedy else torch.empty((n, g, draft.vocab_size), dtype=torch.float32, device=device)
+    for i in range(g + 1):
+        session.launch()
+        if i < g:
+            ids[:, i] = session.next_tokens
+            if qs is not None:
+                qs[:, i] = session.logits
+    for s in slots:
+        cache.commit(s, g + 1)
+    return ids, qs
+
+
+def generate_drafted(model, draft, prompts: Sequence[Sequence[int]], max_tokens: int, params: SamplingParams, drafts: int,
+                     stop_ids=None, context: Optional[int] = None, max_batch: int = 64, cache=None, draft_cache=None,
+                     counts: Optional[dict] = None) -> List[List[int]]:
+    """``generate`` with ``drafts`` tokens drafted a round by ``draft``."""
+    from ..cache import PAGE_TOKENS
+    from .generate import RequestState, plan_batches, round_up
+    if drafts < 1:
+        raise ValueError(f"at least one token is drafted a round, got {drafts}")
+    context = min(context or model.max_positions, model.max_positions, draft.max_positions)
+    stop = frozenset(model.stop_ids if stop_ids is None else stop_ids)
+    for i, p in enumerate(prompts):
+        if len(p) == 0:
+            raise ValueError(f"prompt {i} is empty")
+        if len(p) > context:
+            raise ValueError(f"prompt {i} has {len(p)} tokens, the context holds {context}")
+    # a round may run `drafts` positions past a request's last
+    need = sorted((round_up(min(context, len(p) + max_tokens + drafts), PAGE_TOKENS) for p in prompts), reverse=True)
+    total = max(sum(need[:max_batch]), PAGE_TOKENS)
+    if cache is None:
+        cache = model.new_cache(max_tokens=total, n_slots=max_batch)
+    if draft_cache is None:
+        draft_cache = draft.new_cache(max_tokens=total, n_slots=max_batch)
+    page = cache.page_tokens
+    batches = plan_batches([len(p) for p in prompts], max_tokens + drafts + 1, context, min(max_batch, cache.n_slots, draft_cache.n_slots),
+                           min(cache.n_pages, draft_cache.n_pages) * page, page)
+    states = [RequestState(i, p) for i, p in enumerate(prompts)]
+    sums = {"rounds": 0, "drafted": 0, "kept": 0}
+    for batch in batches:
+        here: dict = {}
+        run_drafted(model, draft, cache, draft_cache, params, [states[i] for i in batch], stop, max_tokens, context, drafts, counts=here)
+        for key in sums:
+            sums[key] += here[key]
+    if counts is not None:
+        counts.update(sums)
+    return [s.produced for s in states]

@@ -37,15 +37,17 @@ class DecoderModel:
         self.stop_ids = tuple(plan.stop_ids)
         self._ring = PinnedRing()
         self._workspace: dict = {}
-        self.weight_bytes = sum(t.numel() * t.element_size() for t in tensors.values())
+        self.weight_bytes = sum(t.numel() * t.element_size() for t in tensors.values()) - getattr(runtime, "saved_bytes", 0)
         self.graph_safe = all(getattr(p, "graph_safe", True) for p in self.assembly.parts())
 
     # ---------------------------------------------------------------- loading
     @classmethod
-    def from_dir(cls, model_dir: str, dtype="bfloat16", device="cuda:0") -> "DecoderModel":
+    def from_dir(cls, model_dir: str, dtype="bfloat16", device="cuda:0", weight_bits: int = 16,
+                 row_bits: int = 16) -> "DecoderModel":
         """Loads config.json and the weights of a model folder; the class of
-        model is chosen by config.json through the registry."""
-        runtime = Runtime.create(dtype, device)
+        model is chosen by config.json through the registry.  ``weight_bits`` 4: the
+        layers' matrices in 4 bits; ``row_bits`` 8: their rows in 8 (``Runtime``)."""
+        runtime = Runtime.create(dtype, device, weight_bits, row_bits)
         if runtime.device.type != "cuda":
             raise RuntimeError("math_utils_b200 runs on a CUDA device only; there is no CPU path")
         runtime.ops.library()                       # fail now, loudly, if the kernels are missing

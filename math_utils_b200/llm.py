@@ -30,6 +30,9 @@ class Options:
     dtype: str = "bfloat16"         # "float32": the true 32-bit path
     max_batch: int = 64             # most sequences that step together in generate()
     profile: bool = False           # prompt() keeps per-stage device times (eager steps; see stage_times)
+    weight_bits: int = 16           # 4: the layers' matrices in 4 bits (with dtype "bfloat16")
+    row_bits: int = 16              # 8: with 4-bit weights, the rows that meet them in 8 bits too
+    drafts: int = 0                 # tokens that the same model in 4 bits drafts a step, for this one to verify
 
 
 class LLM:
@@ -38,9 +41,12 @@ class LLM:
         self.options = replace(options or Options(), **overrides)
         self.device = device
         self.model: Optional[DecoderModel] = None
+        self.draft: Optional[DecoderModel] = None        # with options.drafts: the same weights in 4 bits
+        self.draft_counts: dict = {}    # with options.drafts: rounds, drafted and kept tokens of the last call
         self.current = ""
         self._cache = None
         self._batch_cache = None
+        self._draft_cache = self._draft_slot = None
         self._slot = None
         self._turns = 0
         self.last: dict = {}            # figures of the last prompt(): tokens in and out, seconds, why it ended
@@ -54,13 +60,25 @@ class LLM:
         self.unload()
         if options is not None:
             self.options = options
-        self.model = DecoderModel.from_dir(model_dir, dtype=self.options.dtype, device=self.device)
+        o = self.options
+        if o.drafts < 0 or (o.drafts and (o.dtype != "bfloat16" or o.profile)):
+            raise ValueError("drafted tokens: a number of 0 or more, with dtype bfloat16 and without profile")
+        self.model = DecoderModel.from_dir(model_dir, dtype=o.dtype, device=self.device, weight_bits=o.weight_bits,
+                                           row_bits=o.row_bits)
+        if o.drafts:
+            from .engine.drafted import check_draftable
+            try:
+                self.draft = DecoderModel.from_dir(model_dir, dtype=o.dtype, device=self.device, weight_bits=4, row_bits=o.row_bits)
+                check_draftable(self.model, self.draft, self.model.new_cache(64, 1), self.draft.new_cache(64, 1))
+            except ValueError:
+                self.unload()
+                raise
         self.current = model_dir
         return self
 
     def unload(self) -> None:
         self.model, self._cache, self._slot, self.current, self._turns = None, None, None, "", 0
-        self._batch_cache = None
+        self._batch_cache = self.draft = self._draft_cache = self._draft_slot = None
 
     @property
     def loaded(self) -> bool:
@@ -79,7 +97,9 @@ class LLM:
     def reset(self) -> None:
         if self._slot is not None:
             self._cache.release(self._slot)
-        self._slot, self._turns = None, 0
+        if self._draft_slot is not None:
+            self._draft_cache.release(self._draft_slot)
+        self._slot, self._draft_slot, self._turns = None, None, 0
 
     def prompt(self, ids: Sequence[int], max_tokens: Optional[int] = None) -> List[int]:
         """Feeds ``ids`` after what the conversation already holds and returns
@@ -106,6 +126,10 @@ class LLM:
             raise ValueError("the prompt alone does not fit in the context")
         if self._slot is None:
             self._slot = self._cache.acquire()
+            if self.draft is not None:
+                if self._draft_cache is None:
+                    self._draft_cache = self.draft.new_cache(max_tokens=-(-limit // 64) * 64, n_slots=1)
+                self._draft_slot = self._draft_cache.acquire()
         # the conversation so far counts toward the context rule; the turn keys the sampling stream
         state = RequestState(self._turns, list(ids), held=held)
         self._turns += 1
@@ -114,9 +138,12 @@ class LLM:
             from .engine.stage_timer import StageTimer
             timer = StageTimer()
         try:
-            run_requests(self.model, self._cache, self._params(None, None, None), [state],
-                         frozenset(self.model.stop_ids), max_tokens, limit, kept_slots=[self._slot],
-                         timing=timing, stage_timer=timer)
+            if self.draft is not None:
+                self._prompt_drafted(state, max_tokens, limit, timing)
+            else:
+                run_requests(self.model, self._cache, self._params(None, None, None), [state],
+                             frozenset(self.model.stop_ids), max_tokens, limit, kept_slots=[self._slot],
+                             timing=timing, stage_timer=timer)
         except Exception:
             self.reset()               # the cache may hold half a turn
             raise
@@ -125,6 +152,17 @@ class LLM:
                      "context_used": self._cache.length(self._slot), "context": limit,
                      "prompt_s": timing.get("prompt_s", 0.0), "decode_s": timing.get("decode_s", 0.0)}
         return state.produced
+
+    def _prompt_drafted(self, state, max_tokens: int, limit: int, timing: dict) -> None:
+        import time
+        from .engine.drafted import run_drafted
+        t0, first = time.perf_counter(), []
+        self.draft_counts = {}
+        run_drafted(self.model, self.draft, self._cache, self._draft_cache, self._params(None, None, None), [state],
+                    frozenset(self.model.stop_ids), max_tokens, limit, self.options.drafts,
+                    kept_slots=[(self._slot, self._draft_slot)], first_sample=first, counts=self.draft_counts)
+        t1 = first[0] if first else time.perf_counter()
+        timing["prompt_s"], timing["decode_s"] = t1 - t0, time.perf_counter() - t1
 
     def once(self, ids: Sequence[int], max_tokens: Optional[int] = None) -> List[int]:
         """One self-contained turn: nothing before it is seen, nothing of it is kept."""
@@ -144,6 +182,12 @@ class LLM:
         self._need_model()
         max_tokens = self.options.max_tokens if max_tokens is None else max_tokens
         max_batch = max_batch or self.options.max_batch
+        if self.draft is not None:
+            from .engine.drafted import generate_drafted
+            self.draft_counts = {}
+            return generate_drafted(self.model, self.draft, prompts, max_tokens, self._params(temperature, top_k, seed),
+                                    self.options.drafts, stop_ids=stop_ids, context=self.context, max_batch=max_batch,
+                                    counts=self.draft_counts)
         # One cache serves call after call (and with it the recorded graphs of its batch sizes); a
         # call that needs more room than any before gets a larger one.
         from .cache import PAGE_TOKENS

@@ -176,6 +176,7 @@ class Mixer(Part):
 
     takes_lazy_norm = False          # see FeedForward
     can_overwrite = False
+    takes_rows8 = False              # ``h`` may come in 8 bits (``ops.Q8Rows``): it only goes on to ``Linear`` products
 
     def cache_spec(self):
         return None
@@ -197,6 +198,7 @@ class FeedForward(Part):
     where it can."""
     takes_lazy_norm = False
     can_overwrite = False
+    takes_rows8 = False
 
     def forward(self, h, residual, ctx) -> None:
         raise NotImplementedError

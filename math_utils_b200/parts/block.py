@@ -22,7 +22,8 @@ buffer; the addition to the stream is made by the launch of the NEXT norm (``ops
 x += m * y, then the normed row), also across layers (``StepContext.pending_join``), so the stream is
 read and written once per sublayer.  Extra parts ``scale1`` and ``scale2`` (role ``scale``) multiply the mixer's and
 the feed-forward's result entry by entry, in the same launch; so is the weighted sum of two mixers side by side made
-there (``forward_pair``).
+there (``forward_pair``).  A model whose rows are in 8 bits has the normed row written so by that launch
+(``ops.residual_add_norm_q8``), for a mixer or feed-forward that sets ``takes_rows8``.
 
 ``parallel_pre_norm``: x += mixer(norm1(x)) + feed_forward(norm2(x)), both sublayers reading the SAME x through a
 norm of their own.  Both norms are made before either sublayer adds into the stream (two RMS norms with one eps
@@ -103,6 +104,8 @@ class PreNormBlock(Arrangement):
         if rt.dtype != torch.bfloat16 or not rt.ops.PREFILL_TC or mixer.head_dim != 64:
             return False
         weights = (mixer.qkv.weight, mixer.out.weight, ff.up.weight, ff.down.weight)
+        if any(not isinstance(w, torch.Tensor) for w in weights):        # in 4 bits: part by part
+            return False
         if any(w.dtype != torch.bfloat16 or w.stride(1) != 1 or w.stride(0) % 8 or w.data_ptr() % 16 or w.shape[1] % 8
                for w in weights):
             return False
@@ -187,7 +190,7 @@ class ScaledPreNormBlock(Arrangement):
 
     def forward(self, x, layer, ctx, cache, owns_cache: bool) -> None:
         y = ctx.buffer("sublayer.out", tuple(x.shape), torch.float32)
-        h = self._norm(layer.norm1, x, ctx)
+        h = self._norm(layer.norm1, x, ctx, layer.mixer)
         ctx.note("ln1", h)
         pair = getattr(layer.mixer, "forward_pair", None)
         if pair is not None:
@@ -202,7 +205,7 @@ class ScaledPreNormBlock(Arrangement):
             ctx.flush_join()
             ctx.note("res1", x)
         if not isinstance(layer.feed_forward, NoFeedForward):
-            h = self._norm(layer.norm2, x, ctx)
+            h = self._norm(layer.norm2, x, ctx, layer.feed_forward)
             ctx.note("ln2", h)
             SandwichNormBlock._sublayer(layer.feed_forward, y, h, y, ctx)
             ctx.pending_join = PendingJoin(x, y, self.mult, scale=self._scale(layer, "scale2"))
@@ -216,16 +219,19 @@ class ScaledPreNormBlock(Arrangement):
         return None if part is None else part.weight
 
     @staticmethod
-    def _norm(norm, x, ctx):
-        """The normed stream, with what is still to be added to the stream added by the same launch."""
+    def _norm(norm, x, ctx, taker=None):
+        """The normed stream, with what is still to be added to the stream added by the same launch; in 8 bits where the
+        model's rows are and ``taker`` passes them on to its products alone."""
         if isinstance(norm, RmsNorm) and norm.offset == 0.0 and norm.scale == 1.0 and x.stride(1) == 1:
             pending, ctx.pending_join = ctx.pending_join, None
             if pending is not None and pending.x is not x:
                 ctx.pending_join = pending
                 ctx.flush_join()
                 pending = None
-            out = ctx.buffer("stream.normed", tuple(x.shape), norm.runtime.dtype)
             p = pending if pending is not None else PendingJoin(x, None)
+            if norm.runtime.row_bits == 8 and norm.groups == 1 and getattr(taker, "takes_rows8", False):
+                return norm.runtime.ops.residual_add_norm_q8(x, p.y, p.mult, norm.weight, norm.eps, y2=p.y2, mult2=p.mult2, scale=p.scale)
+            out = ctx.buffer("stream.normed", tuple(x.shape), norm.runtime.dtype)
             return norm.runtime.ops.residual_add_norm(x, p.y, p.mult, norm.weight, norm.eps, out, groups=norm.groups, y2=p.y2,
                                                       mult2=p.mult2, scale=p.scale)
         ctx.flush_join()

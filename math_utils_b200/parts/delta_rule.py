@@ -32,6 +32,7 @@ from .low_rank import LowRank
 
 
 class GatedDeltaMixer(Mixer):
+    takes_rows8 = True
     can_overwrite = True
 
     def __init__(self, spec: PartSpec):

@@ -89,7 +89,7 @@ class TiedHead(Head):
         table = embedding.table()
         if tuple(table.shape) != (self.vocab_size, self.hidden_size):
             raise ValueError("the tied head and the token table disagree on their sizes")
-        self.linear = Linear(table, None, self.runtime)
+        self.linear = Linear(table, None, self.runtime, keep=True)
 
     takes_lazy_norm = True
 
@@ -115,7 +115,7 @@ class LinearHead(Head):
     def bind(self, tensors, runtime):
         super().bind(tensors, runtime)
         from .linear import Linear
-        self.linear = Linear(tensors[self.tensor_name("weight")], None, runtime)
+        self.linear = Linear(tensors[self.tensor_name("weight")], None, runtime, keep=True)
 
     def forward(self, h):
         import torch

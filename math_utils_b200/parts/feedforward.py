@@ -19,6 +19,7 @@ LEARNED_ACTIVATIONS = ("xielu",)
 class DenseFeedForward(FeedForward):
     takes_lazy_norm = True
     can_overwrite = True
+    takes_rows8 = True
 
     def __init__(self, spec: PartSpec):
         super().__init__(spec)
@@ -64,6 +65,7 @@ class GatedFeedForward(FeedForward):
     """down(act(gate h) * (up h)) with three matrices and no biases; ``activation`` is ``silu``, ``gelu_new`` or
     ``gelu``.  The gate and up matrices are stacked, so one product gives both halves of a row."""
     can_overwrite = True
+    takes_rows8 = True
 
     def __init__(self, spec: PartSpec):
         super().__init__(spec)

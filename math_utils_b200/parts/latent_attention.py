@@ -33,6 +33,7 @@ from .position import rotary_frequencies
 
 
 class LatentAttention(Mixer):
+    takes_rows8 = True
     can_overwrite = True
 
     def __init__(self, spec: PartSpec):
@@ -112,7 +113,7 @@ class LatentAttention(Mixer):
         if runtime.dtype == torch.bfloat16 and not self.window and runtime.ops.latent_prompt_ok(self.dim, self.rot_dim,
                                                                                                 self.vdim, self.kv_rank):
             both = torch.cat([t("uk"), t("uv")], dim=0).contiguous()
-            self.expand = Linear(both, None, runtime)
+            self.expand = Linear(both, None, runtime, keep=True)              # (the other form reads the same matrices)
             self.v_up = both[H * self.dim:].view(H, self.vdim, self.kv_rank)        # (held once)
         # (one entry at least, so that the kernels always get a table)
         self.freq_table = torch.tensor(self.freqs or [0.0], dtype=torch.float64).to(torch.float32).to(runtime.device)

@@ -21,6 +21,7 @@ from .linear import Linear
 
 
 class LightningAttention(Mixer):
+    takes_rows8 = True
     can_overwrite = True
 
     def __init__(self, spec: PartSpec):

@@ -21,6 +21,7 @@ from .low_rank import LowRank
 
 
 class GatedLinearAttention(Mixer):
+    takes_rows8 = True
     can_overwrite = True
 
     def __init__(self, spec: PartSpec):

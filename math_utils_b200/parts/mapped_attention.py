@@ -41,6 +41,7 @@ from .position import rotary_frequencies
 
 
 class MappedAttention(Mixer):
+    takes_rows8 = True
     can_overwrite = True
 
     def __init__(self, spec: PartSpec):

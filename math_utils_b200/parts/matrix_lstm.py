@@ -26,6 +26,7 @@ from .linear import Linear
 
 
 class MatrixLstm(Mixer):
+    takes_rows8 = True
     can_overwrite = True
 
     def __init__(self, spec: PartSpec):

@@ -23,6 +23,7 @@ from .linear import Linear
 
 
 class SelectiveScanMixer(Mixer):
+    takes_rows8 = True
     can_overwrite = True
 
     def __init__(self, spec: PartSpec):

@@ -28,6 +28,7 @@ VALUE_MIX = ("none", "source", "blend")
 
 
 class SinkAttention(Mixer):
+    takes_rows8 = True
     can_overwrite = True
 
     def __init__(self, spec: PartSpec):

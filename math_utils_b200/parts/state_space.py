@@ -24,6 +24,7 @@ from .linear import Linear
 
 
 class StateSpaceMixer(Mixer):
+    takes_rows8 = True
     can_overwrite = True
 
     def __init__(self, spec: PartSpec):

@@ -13,7 +13,23 @@ from __future__ import annotations
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
+import numpy as np
 import torch
+
+
+def uniform_draws(seed: int, request: int, first: int, count: int) -> np.ndarray:
+    """Draws ``first`` .. ``first + count - 1`` of a request's stream, float64 in [0, 1): the numbers the sampling kernel
+    draws (splitmix64 of a key made of seed and request)."""
+    mask = (1 << 64) - 1
+
+    def mixed(x):
+        z = (x + 0x9E3779B97F4A7C15) & mask
+        z = ((z ^ (z >> 30)) * 0xBF58476D1CE4E5B9) & mask
+        z = ((z ^ (z >> 27)) * 0x94D049BB133111EB) & mask
+        return z ^ (z >> 31)
+
+    key = mixed((seed & mask) ^ ((request * 0x9E3779B97F4A7C15) & mask))
+    return np.array([(mixed((key + n * 0xD1B54A32D192ED03) & mask) >> 11) * 2.0 ** -53 for n in range(first, first + count)])
 
 
 @dataclass(frozen=True)
