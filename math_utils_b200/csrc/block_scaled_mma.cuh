@@ -6,6 +6,9 @@
 
 namespace mu {
 
+// The LayerNorm that a product makes of its rows: float32 gamma and beta (or null) [K], the rows picked (or null: the first ones).
+struct RowNorm { const float *gamma, *beta; const int* pick; float eps; };
+
 constexpr int BM_E4M3 = 0, BM_E2M1 = 5;         // operand types of the instruction
 
 // Instruction descriptor of kind::mxf8f6f4: type of A at bit 7, of B at bit 10, both K-major, N >> 3 at bit 17, exponent

@@ -204,7 +204,7 @@ _SIGNATURES = {
 
 # Arguments that go to the library as one record (LinearQ4Args in q4_linear.cu, NormQ8Args in q8_rows.cu, VerifyArgs in verify.cu):
 # twenty arguments one by one cost 1.9 us of the host, packed 0.4.
-_LINEAR_Q4_ARGS = struct.Struct("10P3q8i")
+_LINEAR_Q4_ARGS = struct.Struct("13P3q7if")
 _NORM_Q8_ARGS = struct.Struct("8P3q3f3i")
 _VERIFY_ARGS = struct.Struct("8P4qd6i")
 
@@ -1849,21 +1849,29 @@ def residual_add_norm_q8(x: torch.Tensor, y: Optional[torch.Tensor], mult: float
     return Q8Rows(codes, scales)
 
 
-# bfloat16 rows beyond this many need room for their pieces (Q4_CUT_INSIDE in q4_linear.cu: up to it the product's own blocks cut them;
-# 16 x 6,400 x 1,600: 7.4 us in one launch and 9 in two; 32 x 11,264 x 2,048: 16 and 12)
-_Q4_CUT_INSIDE = 16
+# bfloat16 rows beyond this many need room for their pieces (Q4_CUT_INSIDE in q4_linear.cu: up to it the product's own blocks cut them)
+_Q4_CUT_INSIDE = 8
+Q4_NORM_WIDTH = 8192           # the widest LayerNorm that a product makes of its rows (gamma and beta lie beside its ring)
 
 
 def linear_q4(x, weight: Q4Weight, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
               residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
               out_dtype: Optional[torch.dtype] = None, way: int = 0) -> torch.Tensor:
     """act(x @ W^T + bias) + residual with W in 4 bits.  ``x``: bfloat16 [m, k] with unit stride along k (taken as they
-    are: cut into two 8-bit pieces that together hold them), ``Q8Rows``, or a ``NormedInput``.  Sums are float32;
+    are: cut into two 8-bit pieces that together hold them), ``Q8Rows``, or a ``NormedInput`` (of up to 8 rows the norm
+    is made inside the kernel).  Sums are float32;
     ``out`` bfloat16 (the default) or float32; ``bias`` float32 [n], ``residual`` float32 [m, n], which may be ``out``.
     A row that holds an infinity or NaN gives NaN.  ``way``: 0, or which kernel runs: 1 + b the one for few rows (up to
     64) with b blocks a tile (0: the library chooses), -64, -128 or -192 the one for many with tiles that wide."""
-    if isinstance(x, NormedInput):
-        x = x.materialize()
+    norm = None
+    if type(x) is NormedInput:
+        # the LayerNorms of a few rows are made by the product's own blocks
+        if (x.n_rows <= _Q4_CUT_INSIDE and way >= 0 and x._value is None and x.out_dtype == torch.bfloat16 and x.x.dtype == torch.float32
+                and x.x.dim() == 2 and x.x.shape[1] % 8 == 0 and x.x.shape[1] <= Q4_NORM_WIDTH and x.x.stride(1) == 1 and x.x.stride(0) % 4 == 0
+                and (x.x.data_ptr() | x.gamma.data_ptr() | (0 if x.beta is None else x.beta.data_ptr())) % 16 == 0):
+            norm = x
+        else:
+            x = x.materialize()
     codes, w_scales = weight
     if codes.dtype != torch.uint8 or codes.dim() != 2:
         raise KernelError(f"linear_q4: the weight's codes are uint8 [n, kp / 2], got {codes.dtype} {tuple(codes.shape)}")
@@ -1872,7 +1880,15 @@ def linear_q4(x, weight: Q4Weight, bias: Optional[torch.Tensor] = None, act: Opt
     if n < 1 or half < 64 or half % 64:
         raise KernelError(f"linear_q4: the weight's codes are uint8 [n, kp / 2] with kp a multiple of 128, got {tuple(codes.shape)}")
     _check_scaled(codes, w_scales, kp, "linear_q4, weight")
-    if type(x) is Q8Rows:
+    if norm is not None:
+        given, x_scales, m, k, ldx = x.x, None, x.n_rows, x.x.shape[1], x.x.stride(0)
+        if not 0 <= kp - k < 128:
+            raise KernelError(f"linear_q4: normed rows of {k} entries and weights of {kp} (k rounded up to 128) do not agree")
+        if any(t is not None and (t.dtype != torch.float32 or t.numel() != k or not t.is_contiguous()) for t in (x.gamma, x.beta)):
+            raise KernelError("linear_q4: a norm's gamma and beta are contiguous float32 of a row's length")
+        _i32(x.rows, "rows")
+        _on_current_device(given, x.gamma, x.beta, x.rows)
+    elif type(x) is Q8Rows:
         given, x_scales = x
         if given.dtype != torch.float8_e4m3fn or given.dim() != 2 or given.shape[1] != kp:
             raise KernelError(f"linear_q4: rows are float8_e4m3fn [m, {kp}], got {given.dtype} {tuple(given.shape)}")
@@ -1904,13 +1920,14 @@ def linear_q4(x, weight: Q4Weight, bias: Optional[torch.Tensor] = None, act: Opt
     if m == 0:
         return out
     room = None
-    if x_scales is None and (m > _Q4_CUT_INSIDE or way < 0):
-        room = _new(codes, torch.uint8, 2 * m * kp + 2 * (-(-m // 128) * (kp * 4)))
+    if x_scales is None and norm is None and (m > _Q4_CUT_INSIDE or way < 0):
+        room = _new(codes, torch.uint8, -(-m // 128) * 256 * (kp + kp // 32))
     _check(library().mu_linear_q4(_LINEAR_Q4_ARGS.pack(
         given.data_ptr(), 0 if x_scales is None else x_scales.data_ptr(), codes.data_ptr(), w_scales.data_ptr(),
         0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), out.data_ptr(),
-        0 if room is None else room.data_ptr(), status_word(codes.device).data_ptr(), _stream(), ldx, out.stride(0), ldr, m, n, k, kp, code,
-        out_bf16, way, 0)), ("linear_q4({}x{}x{})", m, n, k), launches=1 if room is None else 2)
+        0 if room is None else room.data_ptr(), status_word(codes.device).data_ptr(), _stream(), 0 if norm is None else norm.gamma.data_ptr(),
+        0 if norm is None or norm.beta is None else norm.beta.data_ptr(), 0 if norm is None or norm.rows is None else norm.rows.data_ptr(),
+        ldx, out.stride(0), ldr, m, n, k, kp, code, out_bf16, way, 0.0 if norm is None else norm.eps)), ("linear_q4({}x{}x{})", m, n, k), launches=1 if room is None else 2)
     return out
 
 

@@ -5,14 +5,16 @@
 // from HBM to the tensor cores without passing a register: TMA spreads them to 16 per 16 bytes of shared memory, the
 // instruction multiplies e2m1 by e4m3 and applies both exponents.  Expanding 4-bit codes in registers would cost two
 // instructions a code where an SM takes in 46 codes a clock.
-//   * a tile is 128 rows of W (128 output columns) by all M rows of X: D[128, NB] = W_tile . X^T, NB = M rounded up to 16,
+//   * a tile is 128 rows of W (128 output columns) by all M rows of X: D[128, NB] = W_tile . X^T, NB = M rounded up to 8, 16,
 //     32 or 64; a stage is 128 of k: 8 KB of codes, 512 bytes of exponents, and the rows' share;
 //   * K is cut over the blocks of a cluster (any number up to 8) so that tiles x splits fill the SMs; the partial tiles
 //     meet in distributed shared memory and are added in rank order.  They lie on the stages, which nothing reads once
 //     every block of the cluster has its accumulator;
-//   * bfloat16 rows are two pieces, each e4m3, that together hold them exactly: two products a step into one
-//     accumulator.  Up to 16 rows are cut here, by eight warps, two a stage (every block cuts its own share of k: 1.3 us a
-//     launch at 8 rows where a launch before costs 3); more rows come cut by a launch of their own (q8_rows.cu).
+//   * bfloat16 rows are two pieces, each e4m3, that together hold them exactly: they lie one behind the other,
+//     one instruction multiplies both (up to 32 columns take the instruction 40 cycles, however few they are), and their
+//     accumulators are added where they are read.  Up to 8 rows are cut here, by eight warps, two a stage (every block cuts its own share of k: 1.2 us a
+//     launch at 8 rows, 3.5 at 16, where a launch before costs 1.4); more rows come cut by a launch of their own
+//     (q8_rows.cu).
 //   * the blocks of a tile begin at different places of k (each tile one 128 further on): every block reads the same rows,
 //     and blocks in step would all ask for the same lines at once.
 // Warp 0 copies the weights, warp 6 the rows (or warps 2-9 cut them), warp 1 owns the tensor memory and issues the products,
@@ -25,7 +27,7 @@ namespace mu {
 constexpr int QF_THREADS = 224, QF_THREADS_CUT = 320;
 constexpr int QF_BN = 128, QF_BK = 128;
 constexpr int QF_MAX_SPLIT = 8;               // blocks of a cluster
-constexpr int QF_MAX_CUT = 16;                // bfloat16 rows that are cut here
+constexpr int QF_MAX_CUT = 8;                 // bfloat16 rows that are cut here
 constexpr uint32_t QF_W_BYTES = QF_BN * QF_BK;            // in shared memory: a byte a code
 constexpr uint32_t QF_W_COPIED = QF_BN * QF_BK / 2;       // what the copy of them counts on its barrier: the packed codes
 
@@ -39,7 +41,11 @@ __device__ __forceinline__ void qf_cluster_wait() { asm volatile("barrier.cluste
 
 // COUNT columns of tensor memory, this warp's 32 lanes.
 template <int COUNT> __device__ __forceinline__ void qf_load_columns(uint32_t taddr, uint32_t (&r)[COUNT]) {
-    if constexpr (COUNT == 16) {
+    if constexpr (COUNT == 8) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(taddr));
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    } else if constexpr (COUNT == 16) {
         asm volatile(
             "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
             : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
@@ -63,15 +69,36 @@ template <typename F> __device__ __forceinline__ void qf_with_act(int act, F f) 
     else f(QfAct<ACT_NONE>());
 }
 
-// How the rows come: in 8 bits, as two pieces of a launch before, or in bfloat16 and cut into two pieces here.
-constexpr int QF_EIGHT = 0, QF_PIECES = 1, QF_SIXTEEN = 2;
+// How the rows come: in 8 bits, as two pieces of a launch before (the second NB rows behind the first, in one matrix), or in
+// bfloat16 and cut into two pieces here.
+// QF_NORMED: the rows are LayerNorms, made here: bfloat16((x - mean) / sqrt(var + eps) * gamma + beta) of float32 rows x, cut as any.
+constexpr int QF_EIGHT = 0, QF_PIECES = 1, QF_SIXTEEN = 2, QF_NORMED = 3;
+__host__ __device__ constexpr bool qf_cuts(int mode) { return mode >= QF_SIXTEEN; }
 
 struct QfRows {
-    const unsigned char* scales[2];   // of the rows or their pieces: [tiles of 128 rows][kb][512]
+    const unsigned char* scales;      // of the rows, or of their pieces: one tile of 128 rows, [kb][512]
     const __nv_bfloat16* x;           // QF_SIXTEEN: [M, K] (ldx)
     long long ldx;
     int K, vec;                       // vec: rows in whole, aligned 16-byte pieces
+    // QF_NORMED: float32 rows norm_x [.][K] (ldx), those that `pick` names (or 0 .. M - 1), all in whole, aligned 16-byte pieces
+    const float *norm_x, *gamma, *beta;
+    const int* pick;
+    float eps;
 };
+
+// Eight entries of a normed row, rounded to bfloat16; gamma and beta from the block's shared memory.
+__device__ __forceinline__ uint4 qf_normed_eight(const float4 (&x)[2], const float* gamma, const float* beta, float mean, float inv) {
+    unsigned int w[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float4 g = reinterpret_cast<const float4*>(gamma)[h], b = reinterpret_cast<const float4*>(beta)[h];
+        const __nv_bfloat162 lo = __floats2bfloat162_rn((x[h].x - mean) * inv * g.x + b.x, (x[h].y - mean) * inv * g.y + b.y);
+        const __nv_bfloat162 hi = __floats2bfloat162_rn((x[h].z - mean) * inv * g.z + b.z, (x[h].w - mean) * inv * g.w + b.w);
+        w[2 * h] = *reinterpret_cast<const unsigned int*>(&lo);
+        w[2 * h + 1] = *reinterpret_cast<const unsigned int*>(&hi);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 // Eight bfloat16 of a row from column c on; columns from K on are zeros.
 __device__ __forceinline__ uint4 qf_load_eight(const QfRows& rows, int row, int c) {
@@ -88,20 +115,20 @@ __device__ __forceinline__ uint4 qf_load_eight(const QfRows& rows, int row, int 
 }
 
 // grid.x = tiles * splits: the blocks of a cluster (along x) share a tile and cut K.  Dynamic shared memory, 1,024-byte
-// aligned: per stage W 16 KB and PIECES x (NB x 128 bytes), then per stage the exponents (512 bytes each).  With splits > 1
+// aligned: per stage W 16 KB and PIECES x (NB x 128 bytes), then per stage the exponents (512 bytes a tile).  With splits > 1
 // this block's partial tile and the shares it is sent lie on the stages when they are no longer read.
 template <int NB, int MODE, typename TC>
-__global__ void __launch_bounds__(MODE == QF_SIXTEEN ? QF_THREADS_CUT : QF_THREADS)
-q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x0,
-                   const __grid_constant__ CUtensorMap map_x1, const unsigned char* __restrict__ w_scales, const QfRows rows,
+__global__ void __launch_bounds__(qf_cuts(MODE) ? QF_THREADS_CUT : QF_THREADS)
+q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const unsigned char* __restrict__ w_scales, const QfRows rows,
                    const float* __restrict__ bias, const float* residual, TC* C, int M, int N, int kb_all, long long ldc,
                    long long ldr, int act, int* status, int splits, int stages) {
     constexpr int PIECES = MODE == QF_EIGHT ? 1 : 2;
-    constexpr uint32_t X_BYTES = NB * QF_BK, STAGE = QF_W_BYTES + PIECES * X_BYTES;
-    constexpr uint32_t SCALE_STAGE = (1 + PIECES) * BS_TILE_BYTES;
-    constexpr uint32_t ACC_COLS = NB < 32 ? 32 : NB, SCALE_COLS = 4 * (1 + PIECES);
-    constexpr uint32_t TMEM_COLS = ACC_COLS + 2 * SCALE_COLS <= 64 ? 64 : 128;
-    constexpr int CHUNK = NB < 32 ? 16 : 32;
+    constexpr int NX = PIECES * NB;                       // rows as the instruction sees them: the pieces one behind the other
+    constexpr uint32_t X_PIECE = NB * QF_BK, STAGE = QF_W_BYTES + PIECES * X_PIECE;
+    constexpr uint32_t SCALE_STAGE = 2 * BS_TILE_BYTES;   // a tile of exponents each
+    constexpr uint32_t ACC_COLS = NX < 32 ? 32 : NX, SCALE_COLS = 8;
+    constexpr uint32_t TMEM_COLS = ACC_COLS + 2 * SCALE_COLS <= 64 ? 64 : ACC_COLS + 2 * SCALE_COLS <= 128 ? 128 : 256;
+    constexpr int CHUNK = NB < 32 ? NB : 32;
     extern __shared__ unsigned char qf_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)qf_raw + 1023) & ~(uintptr_t)1023);
     unsigned char* scale_smem = base + (size_t)stages * STAGE;
@@ -109,6 +136,7 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     __shared__ uint64_t full[16], empty[16], acc_full, parts_in;
     __shared__ uint32_t tmem_slot;
     __shared__ float bias_s[QF_BN];
+    __shared__ float stat_s[2][QF_MAX_CUT];               // QF_NORMED: a row's mean and inverse deviation
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = splits > 1 ? (int)qf_cluster_rank() : 0;
@@ -120,9 +148,8 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 
     if (threadIdx.x == 0) {
         tma_prefetch_map(&map_w);
-        if (MODE != QF_SIXTEEN) tma_prefetch_map(&map_x0);
-        if (MODE == QF_PIECES) tma_prefetch_map(&map_x1);
-        for (int s = 0; s < stages; ++s) { mbar_init(&full[s], MODE == QF_SIXTEEN ? 3 : 2); mbar_init(&empty[s], 1); }
+        if (!qf_cuts(MODE)) tma_prefetch_map(&map_x);
+        for (int s = 0; s < stages; ++s) { mbar_init(&full[s], qf_cuts(MODE) ? 3 : 2); mbar_init(&empty[s], 1); }
         mbar_init(&acc_full, 1);
         mbar_init(&parts_in, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -145,7 +172,7 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     // phases are counted on instead of divided out, and addresses and descriptors are added to.  (With i % stages and
     // descriptors made anew a stage took its loader and its issuer about 500 cycles each, more than its bytes.)
     const int turned = tile % my_kb;                      // where this block begins in its share of k
-    if (warp == 0 || (MODE != QF_SIXTEEN && warp == 6)) {
+    if (warp == 0 || (!qf_cuts(MODE) && warp == 6)) {
         const bool weights = warp == 0;
         if (lane == 0) {
             int kb = turned;
@@ -156,13 +183,9 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     tma_load_2d(base + s * STAGE, &map_w, k * QF_BK, n0, &full[s]);
                     bulk_load(scale_smem + s * SCALE_STAGE, w_scales + ((long long)tile * kb_all + k) * BS_TILE_BYTES, BS_TILE_BYTES, &full[s]);
                 } else {
-                    mbar_expect_tx(&full[s], PIECES * (X_BYTES + BS_TILE_BYTES));
-                    tma_load_2d(base + s * STAGE + QF_W_BYTES, &map_x0, k * QF_BK, 0, &full[s]);
-                    bulk_load(scale_smem + s * SCALE_STAGE + BS_TILE_BYTES, rows.scales[0] + (long long)k * BS_TILE_BYTES, BS_TILE_BYTES, &full[s]);
-                    if (MODE == QF_PIECES) {
-                        tma_load_2d(base + s * STAGE + QF_W_BYTES + X_BYTES, &map_x1, k * QF_BK, 0, &full[s]);
-                        bulk_load(scale_smem + s * SCALE_STAGE + 2 * BS_TILE_BYTES, rows.scales[1] + (long long)k * BS_TILE_BYTES, BS_TILE_BYTES, &full[s]);
-                    }
+                    mbar_expect_tx(&full[s], PIECES * X_PIECE + BS_TILE_BYTES);
+                    tma_load_2d(base + s * STAGE + QF_W_BYTES, &map_x, k * QF_BK, 0, &full[s]);
+                    bulk_load(scale_smem + s * SCALE_STAGE + BS_TILE_BYTES, rows.scales + (long long)k * BS_TILE_BYTES, BS_TILE_BYTES, &full[s]);
                 }
                 if (++kb == my_kb) kb = 0;
             };
@@ -186,7 +209,7 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         }
     } else if (warp == 1) {
         const bool one = elect_one();
-        constexpr uint32_t idesc = idesc_block_scaled(BM_E2M1, BM_E4M3, QF_BN, NB);
+        constexpr uint32_t idesc = idesc_block_scaled(BM_E2M1, BM_E4M3, QF_BN, NX);
         const uint64_t w_desc0 = smem_desc_sw128(smem_u32(base)), s_desc0 = scales_desc(smem_u32(scale_smem));
         uint64_t w_desc = w_desc0, s_desc = s_desc0;
         int s = 0;
@@ -197,14 +220,12 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (one) {
                 const uint32_t tmem_s = tmem_acc + ACC_COLS + (i & 1) * SCALE_COLS;      // two sets, in turn
-#pragma unroll
-                for (int p = 0; p <= PIECES; ++p) copy_scales(tmem_s + 4 * p, s_desc + p * (BS_TILE_BYTES / 16));
+                copy_scales(tmem_s, s_desc);
+                copy_scales(tmem_s + 4, s_desc + BS_TILE_BYTES / 16);
 #pragma unroll
                 for (int j = 0; j < QF_BK / 32; ++j)
-#pragma unroll
-                    for (int p = 0; p < PIECES; ++p)
-                        umma_block_scaled(tmem_acc, w_desc + 2 * j, w_desc + (QF_W_BYTES + p * X_BYTES) / 16 + 2 * j,
-                                          idesc | idesc_scale_byte(j), tmem_s, tmem_s + 4 + 4 * p, (i > 0 || j > 0 || p > 0) ? 1u : 0u);
+                    umma_block_scaled(tmem_acc, w_desc + 2 * j, w_desc + QF_W_BYTES / 16 + 2 * j, idesc | idesc_scale_byte(j), tmem_s, tmem_s + 4,
+                                      i > 0 || j > 0 ? 1u : 0u);
                 umma_commit(&empty[s]);
             }
             __syncwarp();
@@ -217,24 +238,72 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     } else {
         const int quad = warp & 3, col = quad * 32 + lane;        // a lane is an output column: n0 + col
         const bool to_bf16 = sizeof(TC) == 2;
-        if (MODE == QF_SIXTEEN) {
+        if (qf_cuts(MODE)) {
             // Two warps take every fourth stage, every other pair of its rows each, a lane eight entries at a time, four neighbours
             // a group of 32: 16 lanes a row.
             constexpr int PAIRS = NB / 4;                          // of rows, a warp
             const int turn = (warp - 2) & 3, pair0 = (warp - 2) >> 2;
             const int half = lane >> 4, c8 = lane & 15;
+            // QF_NORMED: gamma and beta of this block's share of k to shared memory (parameters: before the wait), then a row's mean and
+            // inverse deviation by a warp each
+            float* gamma_s = reinterpret_cast<float*>(scale_smem + (size_t)stages * SCALE_STAGE);
+            float* beta_s = gamma_s + my_kb * QF_BK;
+            if (MODE == QF_NORMED) {
+                for (int j = 4 * ((int)threadIdx.x - 64); j < my_kb * QF_BK; j += 4 * (QF_THREADS_CUT - 64)) {
+                    const int k = kb_begin * QF_BK + j;
+                    const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    *reinterpret_cast<float4*>(gamma_s + j) = k < rows.K ? *reinterpret_cast<const float4*>(rows.gamma + k) : none;
+                    *reinterpret_cast<float4*>(beta_s + j) = rows.beta && k < rows.K ? *reinterpret_cast<const float4*>(rows.beta + k) : none;
+                }
+            }
             pdl_wait();                                            // the rows are the work of earlier kernels
+            if (MODE == QF_NORMED) {
+                const int m = warp - 2;
+                if (m < M) {
+                    const float4* src = reinterpret_cast<const float4*>(rows.norm_x + (long long)(rows.pick ? rows.pick[m] : m) * rows.ldx);
+                    const int n4 = rows.K / 4;
+                    constexpr int KEEP = 13;                       // pieces a lane keeps between the two sums: rows of up to 1,664
+                    float4 v[KEEP];
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < KEEP; ++i) v[i] = lane + 32 * i < n4 ? src[lane + 32 * i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int i = 0; i < KEEP; ++i) sum += (v[i].x + v[i].y) + (v[i].z + v[i].w);
+                    for (int i = lane + 32 * KEEP; i < n4; i += 32) { const float4 x = src[i]; sum += (x.x + x.y) + (x.z + x.w); }
+                    const float mean = warp_sum(sum) / (float)rows.K;
+                    float sq = 0.0f;
+                    auto add = [&](const float4& x) {
+                        const float a = x.x - mean, b = x.y - mean, c = x.z - mean, d = x.w - mean;
+                        sq += (a * a + b * b) + (c * c + d * d);
+                    };
+#pragma unroll
+                    for (int i = 0; i < KEEP; ++i) if (lane + 32 * i < n4) add(v[i]);
+                    for (int i = lane + 32 * KEEP; i < n4; i += 32) add(src[i]);
+                    const float inv = 1.0f / sqrtf(warp_sum(sq) / (float)rows.K + rows.eps);
+                    if (lane == 0) { stat_s[0][m] = mean; stat_s[1][m] = inv; }
+                }
+                asm volatile("bar.sync 2, %0;" ::"n"(QF_THREADS_CUT - 64) : "memory");
+            }
             // Two stages' rows are on their way while a third's are cut.
-            uint4 raw[2][PAIRS];
-            auto ask = [&](int i, int e, uint4& to) {
+            constexpr int WORDS = MODE == QF_NORMED ? 2 : 1;       // 16-byte pieces of eight entries
+            uint4 raw[2][PAIRS][WORDS];
+            auto ask = [&](int i, int e, uint4 (&to)[WORDS]) {
                 const int row = 2 * (2 * e + pair0) + half;
-                to = i < my_kb && row < M ? qf_load_eight(rows, row, (kb_begin + (i + turned < my_kb ? i + turned : i + turned - my_kb)) * QF_BK + 8 * c8)
-                                          : make_uint4(0, 0, 0, 0);
+                const int k = (kb_begin + (i + turned < my_kb ? i + turned : i + turned - my_kb)) * QF_BK + 8 * c8;
+                const bool there = i < my_kb && row < M;
+                if (MODE == QF_NORMED) {
+                    const float* src = there ? rows.norm_x + (long long)(rows.pick ? rows.pick[row] : row) * rows.ldx : nullptr;
+#pragma unroll
+                    for (int h = 0; h < WORDS; ++h)
+                        to[h] = there && k < rows.K ? *reinterpret_cast<const uint4*>(src + k + 4 * h) : make_uint4(0, 0, 0, 0);
+                } else {
+                    to[0] = there ? qf_load_eight(rows, row, k) : make_uint4(0, 0, 0, 0);
+                }
             };
             // (a ring of four stages or more, or of all of them: a warp four stages on then waits for the phase before its own)
             int s = turn % stages;
             uint32_t phase = (uint32_t)(turn / stages) & 1u;
-            auto cut = [&](int i, uint4 (&mine)[PAIRS]) {
+            auto cut = [&](int i, uint4 (&mine)[PAIRS][WORDS]) {
                 if (i >= stages) ok = mbar_wait(&empty[s], phase ^ 1u);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; return; }
                 unsigned char* x0 = base + s * STAGE + QF_W_BYTES;
@@ -243,7 +312,15 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 for (int e = 0; e < PAIRS; ++e) {
                     if (2 * (2 * e + pair0) >= M) break;           // rows past M are left as they are: their columns go nowhere
                     const int row = 2 * (2 * e + pair0) + half;
-                    const unsigned int w[4] = {mine[e].x, mine[e].y, mine[e].z, mine[e].w};
+                    uint4 eight = mine[e][0];
+                    if (MODE == QF_NORMED) {
+                        const int j = (i + turned < my_kb ? i + turned : i + turned - my_kb) * QF_BK + 8 * c8, at_row = row < M ? row : 0;
+                        const float4 x[2] = {make_float4(__uint_as_float(mine[e][0].x), __uint_as_float(mine[e][0].y), __uint_as_float(mine[e][0].z), __uint_as_float(mine[e][0].w)),
+                                             make_float4(__uint_as_float(mine[e][WORDS - 1].x), __uint_as_float(mine[e][WORDS - 1].y), __uint_as_float(mine[e][WORDS - 1].z), __uint_as_float(mine[e][WORDS - 1].w))};
+                        // (columns past K have gamma and beta of 0, whatever the row's mean)
+                        eight = qf_normed_eight(x, gamma_s + j, beta_s + j, stat_s[0][at_row], stat_s[1][at_row]);
+                    }
+                    const unsigned int w[4] = {eight.x, eight.y, eight.z, eight.w};
                     ask(i + 8, e, mine[e]);
                     const unsigned int top = group_top_bf16(w);
                     const bool fine = top < 0x7F80u;
@@ -254,11 +331,10 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     // the copies' layout: 16-byte pieces of a 128-byte row, swapped by the row's place among eight
                     const int at = row * 128 + (((c8 >> 1) ^ (row & 7)) << 4) + (c8 & 1) * 8;
                     *reinterpret_cast<uint2*>(x0 + at) = hi;
-                    *reinterpret_cast<uint2*>(x0 + X_BYTES + at) = lo;
+                    *reinterpret_cast<uint2*>(x0 + X_PIECE + at) = lo;
                     if ((c8 & 3) == 0) {
-                        const int to = (row % 32) * 16 + row / 32 * 4 + c8 / 4;
-                        sx[to] = (unsigned char)b;
-                        sx[BS_TILE_BYTES + to] = (unsigned char)low_exponent(b);
+                        sx[row * 16 + c8 / 4] = (unsigned char)b;
+                        sx[(row + NB) * 16 + c8 / 4] = (unsigned char)low_exponent(b);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // the tensor cores read what was stored here
@@ -291,6 +367,12 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     if (c0 >= M) break;
                     uint32_t r[CHUNK];
                     qf_load_columns<CHUNK>(acc_addr + c0, r);
+                    if (PIECES == 2) {
+                        uint32_t low[CHUNK];
+                        qf_load_columns<CHUNK>(acc_addr + NB + c0, low);
+#pragma unroll
+                        for (int e = 0; e < CHUNK; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) + __uint_as_float(low[e]));
+                    }
                     if (n < N) {
                         float res[CHUNK];                         // all asked for before anything is stored: it may be C itself
 #pragma unroll
@@ -319,6 +401,12 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                     if (c0 >= M) break;
                     uint32_t r[CHUNK];
                     qf_load_columns<CHUNK>(acc_addr + c0, r);
+                    if (PIECES == 2) {
+                        uint32_t low[CHUNK];
+                        qf_load_columns<CHUNK>(acc_addr + NB + c0, low);
+#pragma unroll
+                        for (int e = 0; e < CHUNK; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) + __uint_as_float(low[e]));
+                    }
 #pragma unroll
                     for (int g = 0; g < CHUNK / 4; ++g)
                         if (c0 / 4 + g < groups)
@@ -392,7 +480,7 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 }
 
 template <int NB, int MODE, typename TC>
-static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x0, const CUtensorMap& map_x1, const unsigned char* w_scales,
+static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const unsigned char* w_scales,
                       const QfRows& rows, const float* bias, const float* residual, TC* C, int M, int N, int kb_all, long long ldc,
                       long long ldr, int act, int* status, int splits, int stages, size_t smem, cudaStream_t s) {
     auto kernel = q4_few_rows_kernel<NB, MODE, TC>;
@@ -404,7 +492,7 @@ static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x0, const
     const int tiles = (N + QF_BN - 1) / QF_BN;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * splits));
-    cfg.blockDim = dim3(MODE == QF_SIXTEEN ? QF_THREADS_CUT : QF_THREADS);
+    cfg.blockDim = dim3(qf_cuts(MODE) ? QF_THREADS_CUT : QF_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -423,7 +511,7 @@ static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x0, const
     }
     cfg.attrs = attr;
     cfg.numAttrs = n;
-    return cudaLaunchKernelEx(&cfg, kernel, map_w, map_x0, map_x1, w_scales, rows, bias, residual, C, M, N, kb_all, ldc, ldr, act,
+    return cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, w_scales, rows, bias, residual, C, M, N, kb_all, ldc, ldr, act,
                               status, splits, stages) == cudaSuccess ? MU_OK : MU_ERR_LAUNCH;
 }
 
@@ -471,15 +559,17 @@ static int choose_splits(long long tiles, int kb_all, int rows, int sms) {
     return best;
 }
 
-// W: codes [N, kp / 2] and exponents; kp a multiple of 128 (pointers and strides as mu_linear_q4 has checked them).  The rows: codes x0 [M, kp] with their exponents; or two pieces, x1
-// and its exponents the second; or (x0_scales null, x1 null) bfloat16 x0 [M, K] (ldx) with K > kp - 128, M <= 16.  Codes and
-// exponents 16-byte aligned, W's codes 32-byte.  C bfloat16 or float32 (ldc); residual float32 (ldr), may be C itself.
-// splits: blocks that share a tile and cut K (up to 8; 0: chosen here).  `status` as mu_gemm_tc.
-int launch_q4_few_rows(const void* x0, const void* x0_scales, const void* x1, const void* x1_scales, long long ldx, int K,
-                             const void* w, const void* w_scales, const float* bias, const float* residual, void* C, int M, int N,
-                             int kp, long long ldc, long long ldr, int act, int out_bf16, int splits, int* status, void* stream) {
-    const int mode = !x0_scales ? QF_SIXTEEN : x1 ? QF_PIECES : QF_EIGHT;
-    if (M > (mode == QF_SIXTEEN ? QF_MAX_CUT : 64)) return MU_ERR_UNSUPPORTED_SIZE;
+// The rows of a batch in whole 8s, 16s, 32s or 64s: how far behind the first piece the second one's rows lie.
+int q4_few_rows_tile(int M, bool cut_here) { return cut_here ? 8 : M <= 16 ? 16 : M <= 32 ? 32 : 64; }
+
+// W: codes [N, kp / 2] and exponents (pointers and strides as mu_linear_q4 has checked them); M <= 64.  The rows: 8-bit codes x
+// [M, kp] with one tile of exponents; with two_pieces the second piece's rows q4_few_rows_tile() behind the first's; or
+// (scales null) bfloat16 x [M, K] (ldx), M <= 8; or (norm not null) the LayerNorms of float32 x [.][K] (ldx), M <= 8.  splits: blocks that share a tile and cut K (up to 8; 0: chosen here).
+int launch_q4_few_rows(const void* x, const void* x_scales, bool two_pieces, long long ldx, int K, const void* w, const void* w_scales,
+                       const float* bias, const float* residual, void* C, int M, int N, int kp, long long ldc, long long ldr, int act,
+                       int out_bf16, int splits, const RowNorm* norm, int* status, void* stream) {
+    const int mode = norm ? QF_NORMED : !x_scales ? QF_SIXTEEN : two_pieces ? QF_PIECES : QF_EIGHT;
+    if (M > (qf_cuts(mode) ? QF_MAX_CUT : 64)) return MU_ERR_UNSUPPORTED_SIZE;
     if (splits < 0 || splits > QF_MAX_SPLIT) return MU_ERR_BAD_ARGUMENT;
     const int sms = sm_count();
     if (sms <= 0) return MU_ERR_LAUNCH;
@@ -488,35 +578,45 @@ int launch_q4_few_rows(const void* x0, const void* x0_scales, const void* x1, co
     if (tiles * QF_MAX_SPLIT > 2147483647ll) return MU_ERR_UNSUPPORTED_SIZE;
     if (splits == 0) splits = choose_splits(tiles, kb_all, M, sms);
     if (splits > kb_all) splits = kb_all;
-    const int nb = M <= 16 ? 16 : M <= 32 ? 32 : 64;
-    const size_t operands = QF_W_BYTES + (size_t)pieces * nb * 128, stage_bytes = operands + (1 + pieces) * 512;
+    const int nb = q4_few_rows_tile(M, qf_cuts(mode));
+    const size_t operands = QF_W_BYTES + (size_t)pieces * nb * 128, stage_bytes = operands + 2 * 512;
     // the ring: half of an SM's room where there are blocks for two on one and it leaves each three stages; at least what the
     // partial tiles take
     const size_t parts_bytes = splits > 1 ? (size_t)((M + 3) / 4 * 4 + 4) * 4 * (128 + splits * (128 / splits + 1)) : 0;
     const int per_block = (kb_all + splits - 1) / splits, least = (int)((parts_bytes + operands - 1) / operands);
-    const size_t room = 1024 + 3 * stage_bytes <= 111 * 1024 && tiles * splits > sms ? 111 * 1024 : 220 * 1024;
-    int stages = (int)((room - 1024) / stage_bytes);
+    const size_t norm_bytes = mode == QF_NORMED ? (size_t)per_block * QF_BK * 8 : 0;       // gamma and beta
+    const size_t ring = (qf_cuts(mode) ? 4 : 3) * stage_bytes;
+    const size_t room = 1024 + norm_bytes + ring <= 111 * 1024 && tiles * splits > sms ? 111 * 1024 : 220 * 1024;
+    if (1024 + norm_bytes + ring > room) return MU_ERR_UNSUPPORTED_SIZE;
+    int stages = (int)((room - 1024 - norm_bytes) / stage_bytes);
     if (stages > per_block) stages = per_block;
     if (stages < least) stages = least;
     if (stages > 16) stages = 16;
     if (stages < 1) stages = 1;
-    const size_t smem = 1024 + (size_t)stages * stage_bytes;
-    if (smem > 224 * 1024 || parts_bytes > (size_t)stages * operands || (mode == QF_SIXTEEN && stages < 4 && stages < per_block))
+    const size_t smem = 1024 + (size_t)stages * stage_bytes + norm_bytes;
+    if (smem > 224 * 1024 || parts_bytes > (size_t)stages * operands || (qf_cuts(mode) && stages < 4 && stages < per_block))
         return MU_ERR_UNSUPPORTED_SIZE;
-    CUtensorMap map_w, map_x0 = {}, map_x1 = {};
+    CUtensorMap map_w, map_x = {};
     if (!tensor_map_q4(&map_w, w, N, kp, 128)) return MU_ERR_LAUNCH;
-    if (mode != QF_SIXTEEN && !tensor_map_q8(&map_x0, x0, M, kp, nb)) return MU_ERR_LAUNCH;
-    if (mode == QF_PIECES && !tensor_map_q8(&map_x1, x1, M, kp, nb)) return MU_ERR_LAUNCH;
-    const QfRows rows = {{(const unsigned char*)x0_scales, (const unsigned char*)x1_scales}, (const __nv_bfloat16*)x0, ldx, K,
-                             K % 8 == 0 && ((uintptr_t)x0 & 15) == 0 && (M == 1 || ldx % 8 == 0)};
+    if (!qf_cuts(mode) && !tensor_map_q8(&map_x, x, mode == QF_PIECES ? 2 * nb : M, kp, pieces * nb)) return MU_ERR_LAUNCH;
+    QfRows rows = {(const unsigned char*)x_scales, (const __nv_bfloat16*)x, ldx, K,
+                   K % 8 == 0 && ((uintptr_t)x & 15) == 0 && (M == 1 || ldx % 8 == 0), nullptr, nullptr, nullptr, nullptr, 0.0f};
+    if (norm) {
+        rows.norm_x = (const float*)x;
+        rows.gamma = norm->gamma;
+        rows.beta = norm->beta;
+        rows.pick = norm->pick;
+        rows.eps = norm->eps;
+    }
     cudaStream_t s = (cudaStream_t)stream;
 #define MU_FEW(NB, MODE)                                                                                                            \
-    (out_bf16 ? launch_few<NB, MODE, __nv_bfloat16>(map_w, map_x0, map_x1, (const unsigned char*)w_scales, rows, bias, residual, \
+    (out_bf16 ? launch_few<NB, MODE, __nv_bfloat16>(map_w, map_x, (const unsigned char*)w_scales, rows, bias, residual, \
                                                         (__nv_bfloat16*)C, M, N, kb_all, ldc, ldr, act, status, splits, stages, smem, s) \
-              : launch_few<NB, MODE, float>(map_w, map_x0, map_x1, (const unsigned char*)w_scales, rows, bias, residual, (float*)C, \
+              : launch_few<NB, MODE, float>(map_w, map_x, (const unsigned char*)w_scales, rows, bias, residual, (float*)C, \
                                                 M, N, kb_all, ldc, ldr, act, status, splits, stages, smem, s))
 #define MU_FEW_BOTH(NB) (mode == QF_PIECES ? MU_FEW(NB, QF_PIECES) : MU_FEW(NB, QF_EIGHT))
-    if (mode == QF_SIXTEEN) return MU_FEW(16, QF_SIXTEEN);
+    if (mode == QF_NORMED) return MU_FEW(8, QF_NORMED);
+    if (mode == QF_SIXTEEN) return MU_FEW(8, QF_SIXTEEN);
     if (nb == 16) return MU_FEW_BOTH(16);
     if (nb == 32) return MU_FEW_BOTH(32);
     return MU_FEW_BOTH(64);

@@ -114,10 +114,10 @@ quantize_q4_kernel(const TE* __restrict__ w, long long ldw, int n, int k, int kp
 // ------------------------------------------------------------------------------------------------- rows
 // Eight entries a thread, four neighbouring lanes a group, ROWS rows a thread, all asked for before any is worked on: one where
 // that makes no more blocks than the SMs hold at a time, four for more.
-// PIECES = 2: the second piece's codes lie `m x kp` bytes, its exponents a whole set of tiles, behind the first's.
+// PIECES = 2: the second piece's rows lie `behind` rows behind the first's, in one matrix with one set of exponents.
 template <typename TE, int PIECES, bool VEC, int ROWS>
 __global__ void __launch_bounds__(256)
-quantize_q8_kernel(const TE* __restrict__ x, long long ldx, int m, int k, int kp, unsigned char* __restrict__ codes,
+quantize_q8_kernel(const TE* __restrict__ x, long long ldx, int m, int k, int kp, int behind, unsigned char* __restrict__ codes,
                    unsigned char* __restrict__ scales) {
     pdl_trigger();
     pdl_wait();
@@ -150,19 +150,18 @@ quantize_q8_kernel(const TE* __restrict__ x, long long ldx, int m, int k, int kp
             }
             if (!fine) hi = lo = make_uint2(E4M3_NAN4, E4M3_NAN4);
             *reinterpret_cast<uint2*>(codes + (long long)row * kp + c) = hi;
-            if (PIECES == 2) *reinterpret_cast<uint2*>(codes + ((long long)m + row) * kp + c) = lo;
+            if (PIECES == 2) *reinterpret_cast<uint2*>(codes + ((long long)behind + row) * kp + c) = lo;
         }
         // sixteen lanes hold 128 columns, a word of exponents
         unsigned int word = (unsigned int)b << (8 * (c / BS_GROUP % 4));
         word |= __shfl_xor_sync(0xffffffffu, word, 4);
         word |= __shfl_xor_sync(0xffffffffu, word, 8);
-        if (row < rows && c < kp && c % BS_TILE == 0) {
+        if (row < (PIECES == 2 ? m : rows) && c < kp && c % BS_TILE == 0) {
             unsigned int low = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) low |= (unsigned int)low_exponent(word >> (8 * i) & 255u) << (8 * i);
-            unsigned char* at = scales + scale_at(row, c / BS_GROUP, kp / BS_TILE);
-            *reinterpret_cast<unsigned int*>(at) = word;
-            if (PIECES == 2) *reinterpret_cast<unsigned int*>(at + (long long)rows * (kp / BS_GROUP)) = low;
+            *reinterpret_cast<unsigned int*>(scales + scale_at(row, c / BS_GROUP, kp / BS_TILE)) = word;
+            if (PIECES == 2) *reinterpret_cast<unsigned int*>(scales + scale_at(row + behind, c / BS_GROUP, kp / BS_TILE)) = low;
         }
     }
 }
@@ -263,8 +262,9 @@ MU_EXPORT int mu_quantize_q4(const void* w, long long ldw, int is_bf16, int n, i
 
 namespace mu {
 
-// x [m, k] (ldx) bfloat16 or float32 -> codes [pieces, m, kp], scales [pieces, ceil(m / 128), kp / 128, 512].
-int launch_quantize_q8(const void* x, long long ldx, int is_bf16, int m, int k, int kp, int pieces, void* codes, void* scales, void* stream) {
+// x [m, k] (ldx) bfloat16 or float32 -> codes [m, kp], scales [ceil(m / 128), kp / 128, 512]; behind > 0: two pieces of bfloat16 rows, the
+// second one's rows that many behind the first's (m at least, and both in the same tiles or a multiple of 128).
+int launch_quantize_q8(const void* x, long long ldx, int is_bf16, int m, int k, int kp, int behind, void* codes, void* scales, void* stream) {
     const int rows = (m + 127) / 128 * 128, eights = kp / 8;
     // a block's threads along a row and its rows: whole warps of a row where it has as many eights
     const int along = eights >= 256 ? 256 : eights >= 128 ? 128 : eights >= 64 ? 64 : eights >= 32 ? 32 : 16;
@@ -276,9 +276,9 @@ int launch_quantize_q8(const void* x, long long ldx, int is_bf16, int m, int k, 
     const bool vec = k % 8 == 0 && ((uintptr_t)x & 15) == 0 && (m == 1 || ldx % (is_bf16 ? 8 : 4) == 0);
     cudaStream_t s = (cudaStream_t)stream;
 #define MU_Q8_ROWS(TE, PIECES, VEC, ROWS) \
-    return launch_pdl(quantize_q8_kernel<TE, PIECES, VEC, ROWS>, grid, block, 0, s, 1, (const TE*)x, ldx, m, k, kp, (unsigned char*)codes, (unsigned char*)scales)
+    return launch_pdl(quantize_q8_kernel<TE, PIECES, VEC, ROWS>, grid, block, 0, s, 1, (const TE*)x, ldx, m, k, kp, behind, (unsigned char*)codes, (unsigned char*)scales)
 #define MU_Q8(TE, PIECES, VEC) { if (many) MU_Q8_ROWS(TE, PIECES, VEC, 4); MU_Q8_ROWS(TE, PIECES, VEC, 1); }
-    if (pieces == 2) { if (vec) MU_Q8(__nv_bfloat16, 2, true) MU_Q8(__nv_bfloat16, 2, false) }
+    if (behind > 0) { if (vec) MU_Q8(__nv_bfloat16, 2, true) MU_Q8(__nv_bfloat16, 2, false) }
     if (is_bf16) { if (vec) MU_Q8(__nv_bfloat16, 1, true) MU_Q8(__nv_bfloat16, 1, false) }
     if (vec) MU_Q8(float, 1, true)
     MU_Q8(float, 1, false)
@@ -292,7 +292,7 @@ MU_EXPORT int mu_quantize_q8(const void* x, long long ldx, int is_bf16, int m, i
     if (m <= 0) return MU_OK;
     if (!x || !codes || !scales || k <= 0 || kp % 128 || kp < k || kp - k >= 128 || (m > 1 && ldx < k)) return MU_ERR_BAD_ARGUMENT;
     if (((uintptr_t)codes | (uintptr_t)scales) & 15) return MU_ERR_ALIGNMENT;
-    return mu::launch_quantize_q8(x, m > 1 ? ldx : k, is_bf16, m, k, kp, 1, codes, scales, stream);
+    return mu::launch_quantize_q8(x, m > 1 ? ldx : k, is_bf16, m, k, kp, 0, codes, scales, stream);
 }
 
 // As mu_residual_add_norm with one group, the normed rows in 8 bits: codes [m, kp], scales [ceil(m / 128), kp / 128, 512].  The

@@ -188,6 +188,36 @@ def test_products_into_views_and_into_their_residual(m):
 
 
 @gpu
+@pytest.mark.parametrize("m,n,k", [(1, 130, 8), (3, 300, 104), (8, 200, 1600), (2, 1000, 2048), (5, 129, 4104), (8, 140, 8192), (9, 140, 256), (40, 140, 256)])
+@pytest.mark.parametrize("beta", [True, False])
+def test_products_of_normed_rows(m, n, k, beta):
+    """LayerNorm made inside the product (up to 8 rows) or before it: against the norm in 64 bits, each of whose entries may go
+    either way where it is rounded to bfloat16 (half a step, 2^-8 of it, and the norm's own 32-bit sums)."""
+    x = normal((m + 3, k), 1, 2.0) + 0.7
+    gamma, b = 1.0 + 0.2 * normal((k,), 2), 0.3 * normal((k,), 3) if beta else None
+    weight = ops.quantize_q4(normal((n, k), 4, 0.05).cuda())
+    w = plain.q4_values(u8(weight.codes), u8(weight.scales))[:, :k]
+    pick = torch.randperm(m + 3, generator=torch.Generator().manual_seed(5))[:m].int()
+    for rows in (None, pick):
+        chosen = f64(x if rows is None else x[rows.long()])
+        h = (chosen - chosen.mean(axis=1, keepdims=True)) / np.sqrt(chosen.var(axis=1, keepdims=True) + 1e-5) * f64(gamma)
+        h = h + (f64(b) if beta else 0.0)
+        xs = x.cuda()
+        given = ops.NormedInput(xs, gamma.cuda(), b.cuda() if beta else None, 1e-5, torch.bfloat16, rows=None if rows is None else rows.cuda())
+        got = f64(ops.linear_q4(given, weight, out_dtype=torch.float32))
+        # mean and variance: k roundings at most, of entries up to five times a row's deviation
+        off = product_bound(h, w, torch.float32, 2) + (2.0 ** -8 + (k + 16) * 2.0 ** -24) * (np.abs(h) + 1.0) @ np.abs(w).T
+        assert got.shape == h[:, :1].shape[:1] + (n,) and (np.abs(got - h @ w.T) <= off).all()
+        # bit by bit what the same rows give one at a time
+        one = ops.linear_q4(ops.NormedInput(xs, given.gamma, given.beta, 1e-5, torch.bfloat16,
+                                            rows=torch.tensor([0 if rows is None else int(rows[0])], dtype=torch.int32, device="cuda")), weight,
+                            out_dtype=torch.float32)
+        if given.n_rows <= 8:
+            assert np.array_equal(got[:1], f64(one))
+    ops.check_status()
+
+
+@gpu
 def test_products_give_the_same_bits_again_and_for_a_row_among_others():
     x, w = rough((16, 1600), 1).cuda(), ops.quantize_q4(normal((500, 1600), 2, 0.05).cuda())
     first = ops.linear_q4(x, w, out_dtype=torch.float32)
