@@ -219,9 +219,13 @@ residual_add_norm_q8_kernel(float* __restrict__ x, long long ldx, const Addend a
         const bool fine = is_number(top);
         const int b = fine ? exponent_e4m3(top) : 127;
         const uint2 code = fine ? e4m3_of_eight(v, b) : make_uint2(E4M3_NAN4, E4M3_NAN4);
+        // sixteen lanes hold 128 columns, a word of exponents
+        unsigned int word = (unsigned int)b << (8 * (c / BS_GROUP % 4));
+        word |= __shfl_xor_sync(0xffffffffu, word, 4);
+        word |= __shfl_xor_sync(0xffffffffu, word, 8);
         if (c < kp) {
             *reinterpret_cast<uint2*>(codes + t * kp + c) = code;
-            if (c % BS_GROUP == 0) scales[scale_at(t, c / BS_GROUP, kp / BS_TILE)] = (unsigned char)b;
+            if (c % BS_TILE == 0) *reinterpret_cast<unsigned int*>(scales + scale_at(t, c / BS_GROUP, kp / BS_TILE)) = word;
         }
     };
 #pragma unroll
@@ -231,13 +235,11 @@ residual_add_norm_q8_kernel(float* __restrict__ x, long long ldx, const Addend a
         load_eight<VEC>(xs, c, width, v);                          // written above by this very thread
         put(c, v);
     }
-    // the last row's block gives the tile's rows behind it their (unused) exponents
-    if (t == m - 1) {
-        const long long behind = ((long long)m + BS_TILE - 1) / BS_TILE * BS_TILE - m;
-        const int words = kp / BS_TILE;
-        for (long long i = threadIdx.x; i < behind * words; i += THREADS)
-            *reinterpret_cast<unsigned int*>(scales + scale_at(m + i / words, (int)(i % words) * 4, words)) = 0u;
-    }
+    // the rows behind the last one in its tile get (unused) exponents, every block's share of them
+    const int words = kp / BS_TILE, behind = (m + BS_TILE - 1) / BS_TILE * BS_TILE - m;
+    const unsigned int mine = (int)t < behind ? (unsigned int)((behind - (int)t + m - 1) / m * words) : 0u;
+    for (unsigned int i = threadIdx.x; i < mine; i += THREADS)
+        *reinterpret_cast<unsigned int*>(scales + scale_at(m + t + (long long)(i / words) * m, 4 * (int)(i % words), words)) = 0u;
 }
 
 }  // namespace mu
