@@ -1862,7 +1862,8 @@ def linear_q4(x, weight: Q4Weight, bias: Optional[torch.Tensor] = None, act: Opt
     is made inside the kernel).  Sums are float32;
     ``out`` bfloat16 (the default) or float32; ``bias`` float32 [n], ``residual`` float32 [m, n], which may be ``out``.
     A row that holds an infinity or NaN gives NaN.  ``way``: 0, or which kernel runs: 1 + b the one for few rows (up to
-    64) with b blocks a tile (0: the library chooses), -64, -128 or -192 the one for many with tiles that wide."""
+    64) with b blocks a tile (0: the library chooses), -64, -128, -192 or -256 the one for many with tiles that
+    wide."""
     norm = None
     if type(x) is NormedInput:
         # the LayerNorms of a few rows are made by the product's own blocks

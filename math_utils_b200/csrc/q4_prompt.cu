@@ -7,8 +7,8 @@
 // accumulator, the rate of a bfloat16 product.
 //
 // Persistent: a block an SM walks over the tiles; the ring of stages runs on across tiles, two accumulators in tensor memory
-// take turns, so a tile is read out and stored while the next is multiplied.  192 columns: two accumulators of 256 would
-// leave no tensor memory for the exponents.  Warp 0 copies the rows, warp 10 the weights (one thread cannot issue both in a
+// take turns, so a tile is read out and stored while the next is multiplied.  (Tiles of 256 columns have one: two would
+// leave no tensor memory for the exponents.)  What bounds large products is what an SM takes in from the L2.  Warp 0 copies the rows, warp 10 the weights (one thread cannot issue both in a
 // stage's 384 cycles), warp 1 owns the tensor memory and issues the products, warps 2-9 finish the tiles as in
 // gemm_tc_kernel.cuh.  Waits are bounded as there.
 #include "block_scaled_mma.cuh"
@@ -40,7 +40,8 @@ q4_prompt_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_consta
     typedef QpSmem<BN, PIECES, STAGES> Smem;
     Smem& sm = *reinterpret_cast<Smem*>(((uintptr_t)qp_raw + 1023) & ~(uintptr_t)1023);
     constexpr int W_BLOCKS = BN > 128 ? 2 : 1;                // tiles of exponents that BN columns touch
-    constexpr uint32_t SCALE_COLS = 4 * (PIECES + W_BLOCKS), TMEM_COLS = 2 * BN + 2 * SCALE_COLS <= 256 ? 256 : 512;
+    constexpr int ACCS = BN > 192 ? 1 : 2;                    // accumulators that tensor memory holds beside the exponents
+    constexpr uint32_t SCALE_COLS = 4 * (PIECES + W_BLOCKS), TMEM_COLS = ACCS * BN + 2 * SCALE_COLS <= 256 ? 256 : 512;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int m_tiles = (M + TC_BM - 1) / TC_BM, n_tiles = (N + BN - 1) / BN, tiles = m_tiles * n_tiles;
     bool ok = true;
@@ -117,10 +118,10 @@ q4_prompt_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_consta
         int s = 0, local = 0;
         uint32_t phase = 0, set = 0;
         for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++local) {
-            const int buf = local & 1;
+            const int buf = ACCS == 2 ? local & 1 : 0, turn = ACCS == 2 ? local >> 1 : local;
             // which of the exponents' columns this tile's weights begin at: a tile may begin half-way into 128 rows of W
             const uint32_t w_from = BN % 128 ? (uint32_t)((tile / m_tiles) * BN % BS_TILE / 32) : 0u;
-            ok = mbar_wait(&sm.acc_empty[buf], (uint32_t)(((local >> 1) & 1) ^ 1));
+            ok = mbar_wait(&sm.acc_empty[buf], (uint32_t)((turn & 1) ^ 1));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t tmem_d = tmem_base + (uint32_t)(buf * BN);
@@ -129,7 +130,7 @@ q4_prompt_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_consta
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (one) {
-                    const uint32_t tmem_s = tmem_base + 2 * BN + set * SCALE_COLS;        // two sets, in turn
+                    const uint32_t tmem_s = tmem_base + ACCS * BN + set * SCALE_COLS;        // two sets, in turn
 #pragma unroll
                     for (int p = 0; p < PIECES + W_BLOCKS; ++p) copy_scales(tmem_s + 4 * p, s_desc + p * (BS_TILE_BYTES / 16));
 #pragma unroll
@@ -160,9 +161,9 @@ q4_prompt_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_consta
         pdl_wait();                                           // the residual is the work of earlier kernels, and C may be read by them
         int local = 0;
         for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++local) {
-            const int buf = local & 1;
+            const int buf = ACCS == 2 ? local & 1 : 0, turn = ACCS == 2 ? local >> 1 : local;
             const int row0 = (tile % m_tiles) * TC_BM + quad * 32, n0 = (tile / m_tiles) * BN;
-            ok = mbar_wait(&sm.acc_full[buf], (uint32_t)((local >> 1) & 1));
+            ok = mbar_wait(&sm.acc_full[buf], (uint32_t)(turn & 1));
             if (!ok) {
                 if (lane == 0) atomicExch(status, 3);
                 break;
@@ -236,26 +237,40 @@ static int launch_prompt(const void* x0, const void* x1, const void* w, const Qp
                       bias, residual, C, M, N, kp / QP_BK, ldc, ldr, act, status, bulk_out);
 }
 
-// Rows and weights as launch_q4_few_rows has them (8 bits, or two pieces); any M.  bn: columns of a tile (64, 128, 192; 0: chosen
-// here).
+// The columns of a tile, by the cycles of the waves that its tiles make: a stage of 128 of k takes its products (2 cycles a column
+// and piece) or what it brings in from the L2 (16 KB a piece of rows, 64 bytes a column, the exponents; 55 bytes a cycle
+// and SM), a tile some 300 cycles more, and 1,800 where it is 256 wide: its one accumulator is read out before the next
+// tile's products begin (and with two pieces its ring has two stages).  Microseconds on a B200 for 128, 192 and 256 columns, 8-bit
+// rows: 777 x 4,800 x 1,600 10.1, 11.9, 8.8; 512 x 4,096 x 2,048 7.3, 8.6, 9.3; 1,000 x 6,400 x 1,600 13.6, 12.4, 14.2;
+// 4,096 x 16,384 x 4,096 232, 208, 210; bfloat16 rows: 1,000 x 6,400 x 1,600 22.8, 21.3, 26.7; 4,096 x 16,384 x 4,096 428, 372, 435.
+static int choose_columns(int M, int N, int kb, int pieces, int sms) {
+    int best = 64;
+    long long least = 1ll << 62;
+    for (int b = 64; b <= 256; b += 64) {
+        const long long tiles = (((long long)N + b - 1) / b) * (((long long)M + 127) / 128);
+        const long long products = 2ll * b * pieces, bytes = 16384ll * pieces + 64ll * b + 512ll * (pieces + (b > 128 ? 2 : 1));
+        long long stage = products > bytes / 55 ? products : bytes / 55;
+        if (b == 256 && pieces == 2) stage += stage / 5;
+        const long long cost = (tiles + sms - 1) / sms * (kb * stage + (b == 256 ? 1800 : 300));
+        if (cost < least) { least = cost; best = b; }
+    }
+    return best;
+}
+
+// Rows and weights as launch_q4_few_rows has them (8 bits, or two pieces); any M.  bn: columns of a tile (64, 128, 192, 256; 0:
+// chosen here).
 int launch_q4_prompt(const void* x0, const void* x0_scales, const void* x1, const void* x1_scales, const void* w, const void* w_scales,
                            const float* bias, const float* residual, void* C, int M, int N, int kp, long long ldc, long long ldr, int act,
                            int out_bf16, int bn, int* status, void* stream) {
     const QpScales scales = {{(const unsigned char*)x0_scales, (const unsigned char*)x1_scales}, (const unsigned char*)w_scales};
     const int sms = sm_count();
     if (sms <= 0) return MU_ERR_LAUNCH;
-    if (bn == 0) {
-        long long least = 1ll << 62;
-        for (int b = 64; b <= 192; b += 64) {
-            const long long tiles = (((long long)N + b - 1) / b) * (((long long)M + 127) / 128);
-            const long long cost = (tiles + sms - 1) / sms * (b + 64);
-            if (cost <= least) { least = cost; bn = b; }
-        }
-    }
+    if (bn == 0) bn = choose_columns(M, N, kp / QP_BK, x1 ? 2 : 1, sms);
     cudaStream_t s = (cudaStream_t)stream;
 #define MU_QP(BN, P, ST)                                                                                                            \
     (out_bf16 ? launch_prompt<BN, P, ST, __nv_bfloat16>(x0, x1, w, scales, bias, residual, (__nv_bfloat16*)C, M, N, kp, ldc, ldr, act, status, s) \
               : launch_prompt<BN, P, ST, float>(x0, x1, w, scales, bias, residual, (float*)C, M, N, kp, ldc, ldr, act, status, s))
+    if (bn == 256) return x1 ? MU_QP(256, 2, 2) : MU_QP(256, 1, 3);
     if (bn == 192) return x1 ? MU_QP(192, 2, 3) : MU_QP(192, 1, 4);
     if (bn == 128) return x1 ? MU_QP(128, 2, 3) : MU_QP(128, 1, 5);
     if (bn == 64) return x1 ? MU_QP(64, 2, 4) : MU_QP(64, 1, 6);

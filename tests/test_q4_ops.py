@@ -170,6 +170,32 @@ def test_products(m, n, k, rows):
 
 
 @gpu
+@pytest.mark.parametrize("rows", ["bfloat16", "eight"])
+@pytest.mark.parametrize("m", [1, 8, 12, 40, 64, 150, 300])
+def test_products_by_every_way(m, rows):
+    """Each kernel, however many blocks share a tile and however wide the tiles are, over several tiles and stages."""
+    n, k = 700, 1300
+    x, w = rough((m, k), m), normal((n, k), 2, 0.05)
+    weight = ops.quantize_q4(w.cuda())
+    w_values = plain.q4_values(u8(weight.codes), u8(weight.scales))
+    if rows == "eight":
+        given = ops.quantize_q8(x.cuda())
+        x_values, pieces = plain.q8_values(u8(given.codes), u8(given.scales)), 1
+    else:
+        given, x_values, pieces, w_values = x.cuda(), f64(x), 2, w_values[:, :k]
+    bias = normal((n,), 7)
+    ways = [-64, -128, -192, -256] + ([1 + b for b in range(9)] if m <= 64 else [])
+    for way in ways:
+        got = ops.linear_q4(given, weight, bias=bias.cuda(), out_dtype=torch.float32, way=way)
+        check_product(x_values, w_values, got, bias, None, None, torch.float32, pieces)
+    ops.check_status()
+    with pytest.raises(KernelError, match="bad argument"):
+        ops.linear_q4(given, weight, way=-100)
+    with pytest.raises(KernelError, match="bad argument" if m <= 64 else "unsupported"):
+        ops.linear_q4(given, weight, way=10)
+
+
+@gpu
 @pytest.mark.parametrize("m", [1, 20, 200])
 def test_products_into_views_and_into_their_residual(m):
     """Rows that lie apart, outputs that are columns of a wider buffer, the residual that is the output; what lies
