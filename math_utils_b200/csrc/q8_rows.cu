@@ -167,13 +167,28 @@ quantize_q8_kernel(const TE* __restrict__ x, long long ldx, int m, int k, int kp
 }
 
 // ------------------------------------------------------------------------------------------------- the norm
+// The sum of every thread's v, the same in all of them.
+template <int THREADS>
+__device__ __forceinline__ double sum_of_block(double v, double* scratch) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double all = 0.0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) all += scratch[w];
+    return all;
+}
+
 // A block a row, eight entries a thread and turn; up to KEEP turns stay in registers between the sum and the codes, wider
-// rows are read again from the stream (each entry by the thread that wrote it).
+// rows are read again from the stream (each entry by the thread that wrote it).  A thread's own squares are added in 32 bits,
+// the threads' sums in 64, and an entry times its row's factor and its weight is rounded once: an entry that is off by a bit
+// of its 24 gets its neighbour's code wherever it lies that near the middle of two, one in a million.
 template <int THREADS, int KEEP, bool VEC>
 __global__ void __launch_bounds__(THREADS)
 residual_add_norm_q8_kernel(float* __restrict__ x, long long ldx, const Addend add, const float* __restrict__ weight, float eps,
                             int m, int width, int kp, unsigned char* __restrict__ codes, unsigned char* __restrict__ scales) {
-    __shared__ float scratch[32];
+    __shared__ double scratch[THREADS / 32];
     pdl_trigger();
     pdl_wait();
     const long long t = blockIdx.x;
@@ -209,12 +224,16 @@ residual_add_norm_q8_kernel(float* __restrict__ x, long long ldx, const Addend a
 #pragma unroll
         for (int i = 0; i < 8; ++i) sq = fmaf(v[i], v[i], sq);
     }
-    const float inv = 1.0f / sqrtf(block_sum(sq, scratch) / (float)width + eps);
+    const double exact = rsqrt(sum_of_block<THREADS>((double)sq, scratch) / (double)width + (double)eps);
+    const float inv = (float)exact, inv_rest = (float)(exact - (double)inv);
     auto put = [&](int c, float (&v)[8]) {                         // all four lanes of a group are here together
         float g[8];
         load_eight<VEC>(weight, c, width, g);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * g[i];
+        for (int i = 0; i < 8; ++i) {
+            const float near = v[i] * inv;                         // and what its rounding and inv's left out, then one rounding
+            v[i] = fmaf(near, g[i], fmaf(v[i], inv_rest, fmaf(v[i], inv, -near)) * g[i]);
+        }
         const unsigned int top = group_max(max_of_eight(v));
         const bool fine = is_number(top);
         const int b = fine ? exponent_e4m3(top) : 127;
