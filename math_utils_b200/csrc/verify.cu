@@ -174,7 +174,9 @@ verify_sums_kernel(const VerifyRows rows, const int* __restrict__ drafts, float 
     const float* row = rows.row(r);
     const int begin = (int)((long long)rows.vocab * part / parts), end = (int)((long long)rows.vocab * (part + 1) / parts);
     const float at_draft = threadIdx.x == 0 ? rows.at_draft(r, row, drafts) : 0.0f;
-    const float scale = inv_t * 1.4426950408889634f;                  // exp((l - top) / T) = 2^((l - top) * scale)
+    // exp((l - top) / T) = 2^((l - top) * scale): the difference first, which is exact near the top (l * scale - top * scale in one fma
+    // would carry the rounding of top * scale, 0.3 % of a row's sum at logits of 1,000 and T = 0.01)
+    const float scale = inv_t * 1.4426950408889634f;
     float top = -INFINITY, sum = 0.0f;
     for_share<VS_THREADS>(row, begin, end, [&](const float (&l)[16], int) {
         float most = top;
@@ -183,9 +185,8 @@ verify_sums_kernel(const VerifyRows rows, const int* __restrict__ drafts, float 
         if (most > -INFINITY) {                                       // (else there is nothing yet)
             sum *= fast_exp2((top - most) * scale);
             top = most;
-            const float shift = -top * scale;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sum += fast_exp2(fmaf(l[e], scale, shift));
+            for (int e = 0; e < 16; ++e) sum += fast_exp2((l[e] - top) * scale);
         } else {
 #pragma unroll
             for (int e = 0; e < 16; ++e) sum += l[e] != l[e] ? l[e] : 0.0f;            // a NaN stays one
@@ -869,7 +870,7 @@ MU_EXPORT int mu_verify_drafts(const VerifyArgs* record) {
     const mu::VerifyRows rows = {target, draft, a.target_seq, a.target_row, a.draft_seq, a.draft_row, batch, drafts, vocab};
     cudaStream_t s = (cudaStream_t)stream;
     const bool cuts = !greedy && top_k > 0 && top_k < vocab, listed = cuts && top_k <= mu::VERIFY_LIST;
-    const double inv_t = greedy ? 1.0 : 1.0 / temperature;
+    const double inv_t = greedy ? 1.0 : fmin(1.0 / temperature, 1e300);       // finite: the maximum's own difference of 0 stays 0
     mu::VerifyPart* p = (mu::VerifyPart*)scratch;
     unsigned long long* lists = listed ? (unsigned long long*)(p + n_rows) : nullptr;
     int code;
@@ -889,7 +890,7 @@ MU_EXPORT int mu_verify_drafts(const VerifyArgs* record) {
     } else {
         const dim3 grid((unsigned)n_rows, (unsigned)parts), block(mu::VS_THREADS);
         if (greedy) code = mu::launch_pdl(mu::verify_best_kernel, grid, block, 0, s, 1, rows, parts, p);
-        else code = mu::launch_pdl(mu::verify_sums_kernel, grid, block, 0, s, 1, rows, draft_tokens, (float)inv_t, parts, p);
+        else code = mu::launch_pdl(mu::verify_sums_kernel, grid, block, 0, s, 1, rows, draft_tokens, (float)fmin(inv_t, 1e38), parts, p);
     }
     if (code != MU_OK) return code;
     if (greedy || listed)

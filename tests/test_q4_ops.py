@@ -379,6 +379,39 @@ def test_verification_of_equal_logits():
 
 
 @gpu
+@pytest.mark.parametrize("vocab,top_k", [(517, 0), (6000, 0), (6000, 50)])
+def test_verification_of_logits_far_from_zero(vocab, top_k):
+    """Only differences of logits count: at logits of 1,000 and a temperature of 0.01 a draw a ten-thousandth below or above the
+    border is still decided right."""
+    b = 128
+    logits, draft_logits, drafts, draws = verify_case(b, 1, vocab, 3)
+    logits, draft_logits = (1000.0 + 0.01 * t for t in (logits, draft_logits))
+    want = []
+    for i in range(b):
+        p, q = (plain.softmax_kept(t[i, 0].numpy(), 0.01, top_k) for t in (logits, draft_logits))
+        x = int(np.argmax(q)) if q[drafts[i, 0]] == 0 or p[drafts[i, 0]] == 0 else int(drafts[i, 0])
+        drafts[i, 0] = x
+        ratio = p[x] / q[x]
+        draws[i, 0] = min(ratio * (1 + (1e-4 if i % 2 else -1e-4)), 0.999)
+        want.append(int(draws[i, 0] * q[x] < p[x]))
+    assert 30 < sum(want) < 120
+    _, kept = ops.verify_drafts(logits.cuda(), draft_logits.cuda(), drafts.cuda(), draws.cuda(), 0.01, top_k)
+    assert kept.tolist() == want
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [1e-37, 1e-42, 5e-324])
+@pytest.mark.parametrize("top_k", [0, 40, 700])
+def test_verification_at_the_lowest_temperatures(temperature, top_k):
+    """All of a row's mass lies on its maximum."""
+    logits, draft_logits, drafts, draws = verify_case(6, 3, 5000, 5, near=0.1)
+    drafts = draft_logits.argmax(dim=2).int()
+    tokens, kept = ops.verify_drafts(logits.cuda(), draft_logits.cuda(), drafts.cuda(), draws.cuda(), temperature, top_k)
+    want = ops.verify_drafts(logits.cuda(), None, drafts.cuda(), draws.cuda(), 0.0, 0)
+    assert torch.equal(tokens, want[0]) and torch.equal(kept, want[1])
+
+
+@gpu
 def test_verification_with_masked_logits():
     """-inf and the type's lowest value take a token out; a row that is masked whole, or holds an infinity, gives its first
     maximum, and the rows of other sequences are as ever."""
