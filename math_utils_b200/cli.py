@@ -79,12 +79,15 @@ def main(argv=None) -> int:
         build_parser().print_usage()
         return 1
 
+    if (args.rows8 and not args.q4) or (args.fp32 and (args.q4 or args.drafts)) or (args.profile and args.drafts):
+        print("--rows8 goes with --q4; --q4 and --drafts go without --fp32, --drafts without --profile", file=sys.stderr)
+        return 1
     from .llm import LLM, Options
     t0 = time.time()
     llm = LLM(model_dir, Options(context=args.ctx, max_tokens=args.tokens, temperature=args.temp,
                                  top_k=args.topk, seed=args.seed, dtype="float32" if args.fp32 else "bfloat16",
                                  profile=args.profile, weight_bits=4 if args.q4 else 16,
-                                 row_bits=8 if args.rows8 and args.q4 else 16, drafts=args.drafts))
+                                 row_bits=8 if args.rows8 else 16, drafts=args.drafts))
     if args.stop is not None:
         llm.model.stop_ids = tuple(parse_ids(args.stop))
     load_s = time.time() - t0

@@ -484,11 +484,7 @@ static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const 
                       const QfRows& rows, const float* bias, const float* residual, TC* C, int M, int N, int kb_all, long long ldc,
                       long long ldr, int act, int* status, int splits, int stages, size_t smem, cudaStream_t s) {
     auto kernel = q4_few_rows_kernel<NB, MODE, TC>;
-    static bool raised = false;
-    if (!raised) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024) != cudaSuccess) return MU_ERR_LAUNCH;
-        raised = true;
-    }
+    if (!allow_shared(reinterpret_cast<const void*>(kernel), 224 * 1024)) return MU_ERR_LAUNCH;
     const int tiles = (N + QF_BN - 1) / QF_BN;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * splits));

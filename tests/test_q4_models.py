@@ -8,7 +8,11 @@ import torch
 import plain_gpt2
 import plain_q4 as plain
 import test_forisun_gpu as forisun
+import test_lusalorn_gpu as lusalorn
+import test_pelenex_gpu as pelenex
 import test_seledra_gpu as seledra
+import test_tibopel_gpu as tibopel
+import test_tokolorn_gpu as tokolorn
 from helpers import BF16_NEAR_TIE, check_logits, run_batch, run_tail_one_by_one, run_whole
 from math_utils_b200 import LLM, DecoderModel, Options, write_random_model
 from math_utils_b200.csrc import ops
@@ -93,6 +97,10 @@ class PlainOps:
             z = z + bias
         if act == "gelu_new":
             z = 0.5 * z * (1 + torch.tanh(np.sqrt(2 / np.pi) * (z + 0.044715 * z ** 3)))
+        elif act == "gelu":
+            z = 0.5 * z * (1 + torch.erf(z / np.sqrt(2)))
+        elif act == "relu2":
+            z = z.clamp(min=0) ** 2
         else:
             assert act in (None, "none")
         if residual is not None:
@@ -142,6 +150,56 @@ def test_a_model_of_norms_in_8_bits(name, row_bits, seledra_dirs, monkeypatch):
     # last bit: half a step of e4m3 is 2^-4 of one entry in hundreds, as noise no more than the bfloat16 path's own
     for g, w, what in zip(got, want, ("whole", "tail", "batch")):
         check_logits(g, w, "bfloat16", f"seledra {name} {what}", bf16_rms=seledra.BF16_RMS[name] * (1.5 if row_bits == 8 else 1.0))
+
+
+class CheckedOps(PlainOps):
+    """The kernels themselves, each product and each norm compared with plain torch on the same inputs."""
+
+    def __init__(self, monkeypatch):
+        self.kernels = ops.residual_add_norm_q8, ops.linear_q4
+        super().__init__(monkeypatch)
+
+    def norm(self, x, y, mult, weight, eps, y2=None, mult2=0.0, scale=None):
+        before = x.clone()
+        rows = self.kernels[0](x, y, mult, weight, eps, y2=y2, mult2=mult2, scale=scale)
+        want = super().norm(before, y, mult, weight, eps, y2=y2, mult2=mult2, scale=scale)
+        assert torch.allclose(x, before, rtol=1e-5, atol=1e-6)
+        got, want = ops.q8_values(rows), ops.q8_values(want)
+        # a whole step of e4m3 where an entry lies at an edge between two codes, and for a group's small ones at that of its largest
+        top = want.unflatten(1, (-1, 32)).abs().amax(dim=2, keepdim=True).expand(-1, -1, 32).flatten(1)
+        assert ((got - want).abs() <= 2.0 ** -3 * want.abs() + 2.0 ** -15 * top).all()
+        return rows
+
+    def linear(self, x, weight, bias=None, act=None, residual=None, out=None, out_dtype=None, way=0):
+        given = x.materialize_copy() if isinstance(x, ops.NormedInput) else x
+        res = None if residual is None else residual.clone()
+        got = self.kernels[1](x, weight, bias, act=act, residual=residual, out=out, out_dtype=out_dtype)
+        want = super().linear(given, weight, bias, act, res, None, torch.float64)
+        # half a step of bfloat16 of the answer and of the row's largest sum's own errors
+        assert torch.isfinite(got).all()
+        assert ((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * want.abs().amax(dim=1, keepdim=True)).all()
+        return got
+
+
+FAMILIES = {"forisun": forisun, "lusalorn": lusalorn, "pelenex": pelenex, "seledra": seledra, "tibopel": tibopel, "tokolorn": tokolorn}
+
+
+@gpu
+@pytest.mark.parametrize("name", ["a", "b", "c"])
+@pytest.mark.parametrize("family", FAMILIES)
+def test_every_design_with_4_bit_matrices(family, name, tmp_path, monkeypatch):
+    """What each mixer and feed-forward hands to the products and takes from the norm, in a prompt, a batch and single tokens."""
+    d = write_random_model(str(tmp_path), FAMILIES[family].CONFIGS[name], seed=5)
+    for row_bits in (16, 8):
+        model = DecoderModel.from_dir(d, weight_bits=4, row_bits=row_bits)
+        cache = model.new_cache(max_tokens=4 * 192, n_slots=4)
+        with monkeypatch.context() as patch:
+            checked = CheckedOps(patch)
+            whole = run_whole(model, cache, tokens_for(model.vocab_size, 70, 3))
+            run_tail_one_by_one(model, cache, tokens_for(model.vocab_size, 24, 4), 6)
+            run_batch(model, cache, [tokens_for(model.vocab_size, n, n) for n in (20, 40, 3)], [17, 36, 1])
+        assert checked.products > 0 and np.isfinite(whole).all()
+        ops.check_status()
 
 
 @gpu
@@ -305,3 +363,10 @@ def test_the_command_line_drafts(model_dirs, capsys):
     assert len(drafted) <= 6 and all(t.isdigit() for t in drafted)
     assert main([model_dirs["tiny_a"], "--prompt", "1 2 3", "--tokens", "6", "--temp", "0", "--q4", "--rows8"]) == 0
     assert capsys.readouterr().out.strip()
+
+
+def test_the_command_line_refuses(capsys):
+    from math_utils_b200.cli import main
+    for flags in (["--rows8"], ["--q4", "--fp32"], ["--drafts", "2", "--fp32"], ["--drafts", "2", "--profile"]):
+        assert main(["nowhere", *flags]) == 1
+        assert "--rows8 goes with --q4" in capsys.readouterr().err
