@@ -875,12 +875,17 @@ MU_EXPORT int mu_verify_drafts(const VerifyArgs* record) {
     unsigned long long* lists = listed ? (unsigned long long*)(p + n_rows) : nullptr;
     int code;
     if (listed) {
-        // blocks a row: as many as keep what a share gathers near 1,000 (top_k for every 8,192 logits), and more where there are
-        // few rows; their lists together are what the first of them ranks
+        // blocks a row: as many as keep what a share gathers near 1,000 (top_k for every 8,192 logits), and more where there are few
+        // rows, while every SM gets one at most and a share fills its threads' registers (8,192 logits); their lists together are
+        // what the first of them ranks.  Microseconds with 1, 2, 4, 8 blocks a row, both launches, rows of 50,257 and a top_k of 40:
+        // 9 rows 19.3, 16.4, 15.2, 15.7; 36 rows 19.1, 17.3, 16.0, 21.0; 72 rows 19.7, 17.4, 21.5, 27.5; 288 rows 28, 34, 48, 73; a top_k
+        // of 200, 72 rows: 112, 51, 48, 57.
+        const int sms = mu::sm_count();
+        if (sms <= 0) return MU_ERR_LAUNCH;
         parts = 1;
         int blocks = 1;
         while (blocks < 8 && 2 * blocks * top_k <= mu::VK_MERGE && vocab / (2 * blocks) >= 2 * top_k &&
-               ((long long)vocab / blocks * top_k > 1000ll * 8192 || (n_rows * blocks <= 148 && vocab / (2 * blocks) >= 4096)))
+               ((long long)vocab / blocks * top_k > 1000ll * 8192 || (n_rows * 2 * blocks <= sms && vocab / (2 * blocks) >= mu::VK_HELD * mu::VK_THREADS)))
             blocks *= 2;
         if (n_rows * blocks > 2147483647ll) return MU_ERR_UNSUPPORTED_SIZE;
         code = mu::launch_clusters(mu::verify_top_kernel, (int)n_rows, blocks, mu::VK_THREADS, 0, s, rows, draft_tokens, inv_t, top_k, blocks, p, lists);
