@@ -542,8 +542,8 @@ bool tensor_map_q8(CUtensorMap* map, const void* base, long long rows, int kp, i
 
 // How many blocks share a tile, in units of a stage (0.2 us of an SM when all take in weights).  The exchange of parts costs
 // five stages, one more for every block that takes part and one for 8 rows; a second block on an SM halves both rings.
-// Microseconds on a B200, 8-bit rows: 1 x 6,400 x 1,600 uncut 4.3, by 2 4.5, by 4 4.8; 8 x 1,600 x 6,400 uncut 13.9, by 2 8.2, by
-// 5 5.3, by 8 5.8; 8 x 4,096 x 2,048 uncut 5.3, by 2 4.5, by 4 4.6; 48 x 11,264 x 2,048 uncut 8.7, by 2 10.2, by 4 13.9.
+// Microseconds on a B200, 8-bit rows: 1 x 6,400 x 1,600 uncut 4.0, by 2 4.6, by 4 4.8; 8 x 1,600 x 6,400 uncut 13.4, by 2 8.2, by
+// 5 5.2, by 8 5.8; 8 x 4,096 x 2,048 uncut 4.8, by 2 4.5, by 4 4.6; 48 x 11,264 x 2,048 uncut 8.6, by 2 9.4, by 4 13.4.
 static int choose_splits(long long tiles, int kb_all, int rows, int sms) {
     int best = 1;
     long long least = 1ll << 60;

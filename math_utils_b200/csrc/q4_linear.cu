@@ -13,8 +13,8 @@ int launch_q4_prompt(const void* x0, const void* x0_scales, const void* x1, cons
 int launch_quantize_q8(const void* x, long long ldx, int is_bf16, int m, int k, int kp, int behind, void* codes, void* scales, void* stream);
 
 // Up to 32 rows go to the kernel with the weights as the wide operand; up to 64 where that kernel can cut a long k and the other
-// would leave most SMs idle.  Microseconds, 8-bit rows, that kernel and the other: 8 x 6,400 x 1,600 4.5 and 6.3; 32 x 11,264 x
-// 2,048 7.2 and 9.4; 32 x 6,400 x 1,600 6.1 and 5.8; 64 x 1,600 x 6,400 8.4 and 12.3; 64 x 4,096 x 2,048 9.0 and 5.9.
+// would leave most SMs idle.  Microseconds, 8-bit rows, that kernel and the other: 8 x 6,400 x 1,600 4.1 and 6.0; 32 x 11,264 x
+// 2,048 6.9 and 9.3; 32 x 6,400 x 1,600 5.8 and 5.7; 48 x 1,600 x 6,400 7.2 and 12.0; 64 x 4,096 x 2,048 9.0 and 5.9.
 static bool few_rows(int m, int n, int kp, int sms) {
     return m <= 32 || (m <= 64 && kp >= 32 * 128 && ((long long)n + 127) / 128 * 4 <= sms);
 }
