@@ -540,16 +540,22 @@ bool tensor_map_q8(CUtensorMap* map, const void* base, long long rows, int kp, i
     return tensor_map_codes(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rows, kp, kp, box_rows);
 }
 
-// How many blocks share a tile, in units of a stage (0.2 us of an SM when all take in weights).  The exchange of parts costs
-// five stages, one more for every block that takes part and one for 8 rows; a second block on an SM halves both rings.
+// How many blocks share a tile, in hundredths of a stage of a block alone on its SM (some 0.25 us).  Two blocks on an SM fill each
+// other's waits: their stages take two thirds of that each, but the ring is half as long (three stages more).  The exchange of parts
+// costs five stages, one more for every block that takes part and one for 8 rows.  A cluster lies within one part of the chip: of three to six
+// blocks they fill some 7 of 8 SMs at once, of seven and eight 3 of 4 (16 of eight took 11.6 us where 16 of six took 7.1).
 // Microseconds on a B200, 8-bit rows: 1 x 6,400 x 1,600 uncut 4.0, by 2 4.6, by 4 4.8; 8 x 1,600 x 6,400 uncut 13.4, by 2 8.2, by
-// 5 5.2, by 8 5.8; 8 x 4,096 x 2,048 uncut 4.8, by 2 4.5, by 4 4.6; 48 x 11,264 x 2,048 uncut 8.6, by 2 9.4, by 4 13.4.
+// 5 5.2, by 8 5.8; 8 x 4,096 x 2,048 uncut 4.8, by 2 4.5, by 4 4.6; 48 x 11,264 x 2,048 uncut 8.6, by 2 9.4, by 4 13.4; 8 x 16,384 x
+// 8,192 uncut 18.4, by 2 15.1, by 4 19.8; 8 x 8,192 x 8,192 uncut 17.4, by 2 11.4, by 4 10.2; 8 x 28,672 x 4,096 uncut 13.0, by 2 18.4.
 static int choose_splits(long long tiles, int kb_all, int rows, int sms) {
     int best = 1;
     long long least = 1ll << 60;
     for (int s = 1; s <= QF_MAX_SPLIT && s <= kb_all; ++s) {
-        const long long per_sm = (tiles * s + sms - 1) / sms;                 // blocks that an SM runs, at once or in turn
-        const long long cost = per_sm * ((kb_all + s - 1) / s) + (per_sm > 1 ? 3 : 0) + (s > 1 ? 5 + s + rows / 8 : 0);
+        const int filled = s <= 2 ? sms : s <= 6 ? sms * 7 / 8 : sms * 3 / 4;
+        long long per_sm = (tiles * s + filled - 1) / filled;                 // blocks that an SM runs, two at a time
+        if (per_sm > 1) per_sm = (per_sm + 1) / 2 * 2;
+        const long long stages = per_sm * ((kb_all + s - 1) / s);
+        const long long cost = (per_sm > 1 ? 66 * stages + 300 : 100 * stages) + (s > 1 ? 100 * (5 + s + rows / 8) : 0);
         if (cost < least) { least = cost; best = s; }
     }
     return best;
