@@ -2056,7 +2056,7 @@ def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], dr
     if logits.dtype != torch.float32 or logits.dim() != 3 or logits.stride(2) != 1 or logits.shape[1] < 1 or logits.shape[2] < 1:
         raise KernelError("verify_drafts: logits are float32 [batch, drafts + 1, vocab] with unit inner stride")
     b, g, vocab = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
-    temperature, top_k = float(temperature), max(int(top_k), 0)
+    temperature, top_k = float(temperature), min(max(int(top_k), 0), 2 ** 31 - 1)          # the library's is an int
     if temperature != temperature or temperature == float("inf"):
         raise KernelError(f"verify_drafts: the temperature is a finite number, got {temperature}")
     greedy = temperature <= 0.0 or top_k == 1

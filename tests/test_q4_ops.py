@@ -465,6 +465,14 @@ def test_verification_of_strided_logits():
 
 
 @gpu
+@pytest.mark.parametrize("top_k", [700, 2 ** 31 - 1, 2 ** 31, 2 ** 40, -2 ** 40])
+def test_verification_with_a_top_k_past_the_vocabulary(top_k):
+    dev = [t.cuda() for t in verify_case(6, 3, 700, 11)]
+    got, want = ops.verify_drafts(*dev, 0.9, top_k), ops.verify_drafts(*dev, 0.9, 0)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@gpu
 def test_verified_tokens_are_distributed_as_the_target():
     """The first token of 20,000 independent sequences of one draft, over a vocabulary of 6: frequencies against the target's
     probabilities (a binomial count is within 5 of its standard deviations but for one in a million)."""
