@@ -182,10 +182,18 @@ __device__ __forceinline__ double sum_of_block(double v, double* scratch) {
     return all;
 }
 
+__device__ __forceinline__ double squares_of_eight(const float (&v)[8]) {
+    const float a = fmaf(v[0], v[0], v[1] * v[1]), b = fmaf(v[2], v[2], v[3] * v[3]);
+    const float c = fmaf(v[4], v[4], v[5] * v[5]), d = fmaf(v[6], v[6], v[7] * v[7]);
+    return (double)((a + b) + (c + d));
+}
+
 // A block a row, eight entries a thread and turn; up to KEEP turns stay in registers between the sum and the codes, wider
-// rows are read again from the stream (each entry by the thread that wrote it).  A thread's own squares are added in 32 bits,
-// the threads' sums in 64, and an entry times its row's factor and its weight is rounded once: an entry that is off by a bit
-// of its 24 gets its neighbour's code wherever it lies that near the middle of two, one in a million.
+// rows are read again from the stream (each entry by the thread that wrote it).  Eight squares are added pairwise in 32 bits (the
+// row's factor is off by 2^-23 of itself at most), the eights in 64, and an entry times its row's factor and its weight is
+// rounded once: an entry that is off by a bit of its 24 gets its neighbour's code wherever it lies that near the middle of two.
+// With a thread's 32 squares on one 32-bit sum a row with a few large entries lost the small ones, and twice as many codes of
+// ordinary rows went to the neighbour.
 template <int THREADS, int KEEP, bool VEC>
 __global__ void __launch_bounds__(THREADS)
 residual_add_norm_q8_kernel(float* __restrict__ x, long long ldx, const Addend add, const float* __restrict__ weight, float eps,
@@ -196,7 +204,7 @@ residual_add_norm_q8_kernel(float* __restrict__ x, long long ldx, const Addend a
     const long long t = blockIdx.x;
     float* xs = x + t * ldx;
     float kept[KEEP][8];
-    float sq = 0.0f;
+    double sq = 0.0;
     auto take = [&](int c, float (&v)[8]) {                        // the stream's entries with the addition made
         load_eight<VEC>(xs, c, width, v);
         if (!add.y || c >= width) return;
@@ -217,16 +225,14 @@ residual_add_norm_q8_kernel(float* __restrict__ x, long long ldx, const Addend a
     for (int j = 0; j < KEEP; ++j) {
         const int c = 8 * (threadIdx.x + j * THREADS);
         take(c, kept[j]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sq = fmaf(kept[j][i], kept[j][i], sq);
+        sq += squares_of_eight(kept[j]);
     }
     for (int c = 8 * (threadIdx.x + KEEP * THREADS); c < width; c += 8 * THREADS) {
         float v[8];
         take(c, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sq = fmaf(v[i], v[i], sq);
+        sq += squares_of_eight(v);
     }
-    const double exact = rsqrt(sum_of_block<THREADS>((double)sq, scratch) / (double)width + (double)eps);
+    const double exact = rsqrt(sum_of_block<THREADS>(sq, scratch) / (double)width + (double)eps);
     const float inv = (float)exact, inv_rest = (float)(exact - (double)inv);
     auto put = [&](int c, float (&v)[8]) {                         // all four lanes of a group are here together
         float g[8];

@@ -309,6 +309,29 @@ def test_norm_with_rows_in_eight_bits(m, k):
 
 
 @gpu
+@pytest.mark.parametrize("k", [1024, 2048, 4096, 8192, 8200, 16384])
+def test_norm_of_rows_with_a_few_large_entries(k):
+    """Every eighth entry of the first 2,048 is 4,096, the rest are 1: a sum of squares in 32 bits that runs over all of a thread's
+    entries loses each 1 beside 2^24.  Entries lie 4e-7, less their weight's rounding of 2^-24, above and below the middle of two
+    codes; the row's factor may be off by 2^-23 (the squares of eight and their sum: four roundings of 2^-24, half of that in the
+    root) and the entry's one rounding is 2^-24: 1.8e-7 of 3.4e-7, so every code has to be the 64-bit formula's."""
+    x = torch.ones(3, k)
+    x[:, 8 * torch.arange(min(k // 8, 256))] = 4096.0
+    h0 = f64(x) / np.sqrt((f64(x) ** 2).mean(axis=1, keepdims=True) + 1e-5)
+    # middles of two codes between 256 and 416 at a scale of 1, in turn above and below; each group's first entry is 430
+    middles = np.array([272.0, 304.0, 336.0, 368.0, 400.0])
+    column = np.arange(k)
+    want = middles[column % 5] * np.where(column // 5 % 2 == 0, 1 + 4e-7, 1 - 4e-7)
+    want[::32] = 430.0
+    weight = torch.from_numpy(want / h0[0]).float()
+    xs = x.cuda()
+    rows = ops.residual_add_norm_q8(xs, None, 1.0, weight.cuda(), 1e-5)
+    values, e = plain.q8_of(h0 * f64(weight))
+    assert np.array_equal(plain.scale_bytes(u8(rows.scales), 3) - 127.0, e)
+    assert np.array_equal(plain.e4m3(u8(rows.codes)), values)
+
+
+@gpu
 def test_norm_of_strided_and_unaligned_rows():
     buf, other = normal((7, 700), 1).cuda(), normal((7, 700), 2).cuda()
     weight = 1.0 + 0.3 * normal((512,), 4)
