@@ -20,7 +20,8 @@
 // which the first reads 1.5, finds the floor 1.2, gathers 1.7, ranks 1, joins 2.6.
 // The walk is in 64 bits, exponentials included: with 50,000 tokens in a row a running sum that is off by 1e-7 of the whole
 // would give another token once in a hundred draws.  The exponentials are made by a table
-// (exp_of).
+// (exp_of).  Decisions about drafts are the 64-bit formula's too: the first launch's 32-bit sums decide where their error cannot matter, and
+// a draft nearer than that to its border (5e-5 of it, about one in 20,000) has its two rows added up again in 64 bits.
 #include "common.cuh"
 
 #include <cooperative_groups.h>
@@ -160,11 +161,21 @@ verify_best_kernel(const VerifyRows rows, int parts, VerifyPart* __restrict__ ou
     }
 }
 
-// 2^x within 2^-22 of itself: for sums that decide about a draft, not about where a draw falls.
+// 2^x within 2^-22 of itself: for sums that decide about a draft where it is not near, not about where a draw falls.
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// How far u q has to lie from p, as a share of the larger, for the sums below to decide about a draft.  A sum's relative error, to first
+// order, in units of 2^-22: an argument is made with five roundings and off by 5 x 2^-24 nats, x its distance from the top
+// in nats, which under a softmax over n < 2^31 tokens averages less than ln n < 22: 28; the exponential itself and the thread's last one: 2;
+// in each of a thread's turns (of 16 logits and one rescaling) 16 additions of 2^-24, one exponential, one product: 6.  Both
+// rows' together, and a quarter more.  Beyond 1e30 for 1 / T the factor in 32 bits is no longer the one in 64: nothing is decided here.
+__host__ inline double margin_of_sums(double inv_t, int vocab, int parts) {
+    const double turns = vocab / parts / (16 * 256) + 2;
+    return inv_t > 1e30 ? 4.0 : 2.5 * (30.0 + 6.0 * turns) / 4194304.0;
 }
 
 // Block (r, part): the part's maximum and its sum.  A thread takes sixteen logits at a time onto its running maximum.
@@ -490,39 +501,86 @@ __device__ __forceinline__ VerifyRow row_of(const VerifyRows& rows, const Verify
 
 constexpr int VERIFY_ROWS = 32;           // rows whose numbers a block keeps
 
-// Decides how many drafts of sequence b are taken, by the block's warps, a place each: one half of a warp has the target's row,
-// the other the draft's.  kept_s: a shared word; kept_rows: shared room for VERIFY_ROWS pairs.  Gives the number and the
-// row pair (p, q) of the place behind the drafts taken; q is p where there is no draft.
-__device__ __forceinline__ int decide(const VerifyRows& rows, const VerifyPart* parts_of, int parts, const int* mine, const double* u, int b,
-                                      double inv_t, int greedy, const double* table, int* kept_s, VerifyRow (*kept_rows)[2], VerifyRow& p,
-                                      VerifyRow& q, bool& ended) {
-    const int g = rows.drafts, lane = threadIdx.x & 31, t0 = b * (g + 1), d0 = rows.batch * (g + 1) + b * g;
-    if (threadIdx.x == 0) *kept_s = g;
-    __syncthreads();
-    for (int i = threadIdx.x >> 5; i <= g; i += blockDim.x >> 5) {
-        const int x = i < g ? mine[i] : -1;
-        const bool theirs = lane >= 16 && !greedy && i < g;
-        const VerifyRow v = row_of(rows, parts_of, theirs ? d0 + i : t0 + i, parts, inv_t, table);
-        if ((lane & 15) == 0 && i < VERIFY_ROWS) kept_rows[i][lane >> 4] = v;
-        bool taken = x >= 0 && x < rows.vocab;
-        if (greedy) taken = taken && x == v.first_best;
-        else {
-            const double m = taken ? v.mass(v.at_draft, x, inv_t, table) * v.inv_sum : 0.0;
-            const double other = __shfl_sync(0xffffffffu, m, 16);
-            taken = taken && u[i] * other < m;             // (lane 0's m is p)
+// A block's sums of exp((l - top) / T) over all of two rows, in 64 bits; the same in every thread, and in every block that makes them.
+__device__ __forceinline__ double2 sums_of_rows(const VerifyRow& p, const VerifyRow& q, int vocab, double inv_t, const double* table,
+                                                double2* scratch) {
+    double sp = 0.0, sq = 0.0;
+    constexpr int U = 4;
+    for (int i0 = threadIdx.x; i0 < vocab; i0 += U * blockDim.x) {
+        float lp[U], lq[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const long long i = (long long)i0 + j * (int)blockDim.x;
+            lp[j] = i < vocab ? p.row[i] : -INFINITY;
+            lq[j] = i < vocab ? q.row[i] : -INFINITY;
         }
-        if (lane == 0 && !taken) atomicMin(kept_s, i);
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const bool there = (long long)i0 + j * (int)blockDim.x < vocab;
+            sp += there ? exp_of(((double)lp[j] - p.top) * inv_t, table) : 0.0;
+            sq += there ? exp_of(((double)lq[j] - q.top) * inv_t, table) : 0.0;
+        }
     }
+    sp = warp_total(sp);
+    sq = warp_total(sq);
+    __syncthreads();                                       // (what the scratch held before has been read)
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = make_double2(sp, sq);
     __syncthreads();
-    const int kept = *kept_s;
-    ended = kept == g || mine[kept] < 0 || mine[kept] >= rows.vocab;       // no draft there: from p alone
-    if (kept < VERIFY_ROWS) {
-        p = kept_rows[kept][0];
-        q = kept_rows[kept][1];
-    } else {
-        p = row_of(rows, parts_of, t0 + kept, parts, inv_t, table);
-        q = ended || greedy ? p : row_of(rows, parts_of, d0 + kept, parts, inv_t, table);
+    double2 all = make_double2(0.0, 0.0);
+    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) { all.x += scratch[w].x; all.y += scratch[w].y; }
+    return all;
+}
+
+// Decides how many drafts of sequence b are taken, by the block's warps, a place each: one half of a warp has the target's row,
+// the other the draft's.  first_s: a shared word; kept_rows: shared room for VERIFY_ROWS pairs.  Gives the number and the
+// row pair (p, q) of the place behind the drafts taken; q is p where there is no draft.
+// MARGIN: the rows' sums are of 32-bit exponentials (verify_sums_kernel), and where u q lies within `margin` of p, as a share of the larger,
+// the place's sums are made again in 64 bits by the whole block, so that every decision is the 64-bit formula's.
+template <bool MARGIN>
+__device__ __forceinline__ int decide(const VerifyRows& rows, const VerifyPart* parts_of, int parts, const int* mine, const double* u, int b,
+                                      double inv_t, int greedy, double margin, const double* table, int* first_s, double2* scratch,
+                                      VerifyRow (*kept_rows)[2], VerifyRow& p, VerifyRow& q, bool& ended) {
+    const int g = rows.drafts, lane = threadIdx.x & 31, t0 = b * (g + 1), d0 = rows.batch * (g + 1) + b * g;
+    auto pair_at = [&](int i, bool both) {                 // all threads, of a place up to g
+        if (i < VERIFY_ROWS) {
+            p = kept_rows[i][0];
+            q = kept_rows[i][1];
+        } else {
+            p = row_of(rows, parts_of, t0 + i, parts, inv_t, table);
+            q = both ? row_of(rows, parts_of, d0 + i, parts, inv_t, table) : p;
+        }
+    };
+    int kept = 0;
+    for (int from = 0;;) {
+        if (threadIdx.x == 0) *first_s = 2 * g;
+        __syncthreads();
+        for (int i = from + (threadIdx.x >> 5); i <= g; i += blockDim.x >> 5) {
+            const int x = i < g ? mine[i] : -1;
+            const bool theirs = lane >= 16 && !greedy && i < g;
+            const VerifyRow v = row_of(rows, parts_of, theirs ? d0 + i : t0 + i, parts, inv_t, table);
+            if ((lane & 15) == 0 && i < VERIFY_ROWS) kept_rows[i][lane >> 4] = v;
+            bool taken = x >= 0 && x < rows.vocab, near = false;
+            if (greedy) taken = taken && x == v.first_best;
+            else {
+                const double m = taken ? v.mass(v.at_draft, x, inv_t, table) * v.inv_sum : 0.0;
+                const double other = u[i] * __shfl_sync(0xffffffffu, m, 16);        // (lane 0's m is p)
+                near = MARGIN && taken && fabs(other - m) < margin * fmax(other, m);
+                taken = taken && other < m;
+            }
+            if (lane == 0 && (near || !taken)) atomicMin(first_s, 2 * i + (near ? 1 : 0));
+        }
+        __syncthreads();
+        const int first = *first_s;                        // the first place that is refused, or too near to say
+        kept = first >> 1;
+        if (!MARGIN || !(first & 1)) break;
+        pair_at(kept, true);
+        const double2 sums = sums_of_rows(p, q, rows.vocab, inv_t, table, scratch);
+        const double mp = p.mass(p.at_draft, mine[kept], inv_t, table) / sums.x, mq = q.mass(q.at_draft, mine[kept], inv_t, table) / sums.y;
+        if (!(u[kept] * mq < mp)) break;
+        from = kept + 1;                                   // (the sums' barriers lie behind everyone's look at first_s)
     }
+    ended = kept == g || mine[kept] < 0 || mine[kept] >= rows.vocab;       // no draft there: from p alone
+    pair_at(kept, !ended && !greedy);
     return kept;
 }
 // The answer's row apart from the drawn token: the drafts taken, -1 behind the token.
@@ -541,7 +599,7 @@ verify_list_kernel(const VerifyRows rows, const VerifyPart* __restrict__ parts_o
                    int top_k, const int* __restrict__ drafts, const double* __restrict__ draws, double inv_t, int greedy,
                    int* __restrict__ tokens, int* __restrict__ kept_out) {
     __shared__ double table[64];
-    __shared__ int kept_s, found_s;
+    __shared__ int first_s, found_s;
     __shared__ int p_at[VERIFY_LIST], q_at[VERIFY_LIST];
     __shared__ double p_mass[VERIFY_LIST], q_mass[VERIFY_LIST], sorted[VERIFY_LIST];
     __shared__ int sorted_at[VERIFY_LIST];
@@ -555,7 +613,7 @@ verify_list_kernel(const VerifyRows rows, const VerifyPart* __restrict__ parts_o
     __syncthreads();
     VerifyRow p, q;
     bool ended;
-    const int kept = decide(rows, parts_of, parts, mine, u, b, inv_t, greedy, table, &kept_s, kept_rows, p, q, ended);
+    const int kept = decide<false>(rows, parts_of, parts, mine, u, b, inv_t, greedy, 0.0, table, &first_s, nullptr, kept_rows, p, q, ended);
     write_taken(rows, mine, kept, b, tokens, kept_out);
     const int pr = b * (g + 1) + kept, qr = rows.batch * (g + 1) + b * g + kept;
     int* out = tokens + (long long)b * (g + 1) + kept;
@@ -630,13 +688,14 @@ constexpr int VW_THREADS = 512, VW_WARPS = VW_THREADS / 32, VW_BLOCKS = 8;
 template <bool CUT, int HELD>
 __global__ void __launch_bounds__(VW_THREADS, 2)
 verify_walk_kernel(const VerifyRows rows, const VerifyPart* __restrict__ parts_of, int parts, const int* __restrict__ drafts,
-                   const double* __restrict__ draws, double inv_t, int blocks, int* __restrict__ tokens, int* __restrict__ kept_out) {
+                   const double* __restrict__ draws, double inv_t, double margin, int blocks, int* __restrict__ tokens, int* __restrict__ kept_out) {
     __shared__ double table[64];
     __shared__ double span_p[VW_WARPS], span_r[VW_WARPS];
+    __shared__ double2 again[VW_WARPS];
     __shared__ double share[4];                            // this block's sums: p, q, then what the token is drawn from
     __shared__ unsigned long long best_s[VW_WARPS];
     __shared__ VerifyRow kept_rows[VERIFY_ROWS][2];
-    __shared__ int kept_s;
+    __shared__ int first_s;
     extern __shared__ double2 held_masses[];               // [HELD][VW_THREADS]
     cg::cluster_group cluster = cg::this_cluster();
     pdl_trigger();
@@ -649,7 +708,7 @@ verify_walk_kernel(const VerifyRows rows, const VerifyPart* __restrict__ parts_o
     __syncthreads();
     VerifyRow p, q;
     bool ended;
-    const int kept = decide(rows, parts_of, parts, mine, u, b, inv_t, 0, table, &kept_s, kept_rows, p, q, ended);      // the same in every block
+    const int kept = decide<!CUT>(rows, parts_of, parts, mine, u, b, inv_t, 0, margin, table, &first_s, again, kept_rows, p, q, ended);      // the same in every block
     if (rank == 0) write_taken(rows, mine, kept, b, tokens, kept_out);
     const int begin = (int)((long long)vocab * rank / blocks), end = (int)((long long)vocab * (rank + 1) / blocks);
     const int w0 = begin + (int)((long long)(end - begin) * warp / VW_WARPS), w1 = begin + (int)((long long)(end - begin) * (warp + 1) / VW_WARPS);
@@ -905,6 +964,7 @@ MU_EXPORT int mu_verify_drafts(const VerifyArgs* record) {
     if (greedy || listed)
         return mu::launch_pdl(mu::verify_list_kernel, dim3((unsigned)batch), dim3(mu::VL_THREADS), 0, s, 1, rows, (const mu::VerifyPart*)p, parts,
                               (const unsigned long long*)lists, top_k, draft_tokens, draws, inv_t, (int)greedy, tokens, kept);
+    const double margin = cuts ? 0.0 : mu::margin_of_sums(inv_t, vocab, parts);
     // Eight blocks a sequence hold the masses of 53,000 tokens in their shared memory (104 KB, two on an SM); a larger vocabulary
     // is read in each pass.
     const int blocks = mu::VW_BLOCKS, held = (vocab / blocks / mu::VW_WARPS + 1 + 31) / 32;
@@ -914,7 +974,7 @@ MU_EXPORT int mu_verify_drafts(const VerifyArgs* record) {
         auto kernel = mu::verify_walk_kernel<CUT, HELD>;                                                                            \
         if (!mu::allow_shared(reinterpret_cast<const void*>(kernel), smem)) return MU_ERR_LAUNCH;                                   \
         return mu::launch_clusters(kernel, batch, blocks, mu::VW_THREADS, smem, s, rows, (const mu::VerifyPart*)p, parts, draft_tokens, draws, \
-                                   inv_t, blocks, tokens, kept);                                                                    \
+                                   inv_t, margin, blocks, tokens, kept);                                                                    \
     } while (0)
     if (cuts) {
         if (held <= 13) MU_WALK(true, 13);

@@ -423,6 +423,26 @@ def test_verification_of_logits_far_from_zero(vocab, top_k):
 
 
 @gpu
+@pytest.mark.parametrize("b,g,vocab,temperature,top_k", [(15, 4, 50257, 1.0, 0), (60, 4, 50257, 0.7, 0), (6, 2, 50257, 0.3, 40), (30, 4, 1031, 1.3, 0),
+                                                         (6, 2, 40000, 0.01, 0), (3, 1, 50257, 1.0, 1000), (41, 40, 300, 1.0, 0)])
+def test_verification_decides_in_64_bits(b, g, vocab, temperature, top_k):
+    """Draws a thousand-millionth below the border take a draft, as far above it refuse it, several in a sequence.  The kernel's
+    exponentials are within 1e-13 (and a sum of n of them within n 2^-53), the statement's within a few 2^-53: an error of 1e-11 at most."""
+    logits, draft_logits, drafts, draws = verify_case(b, g, vocab, 21)
+    if temperature < 0.1:
+        logits, draft_logits = (500.0 + 0.01 * t for t in (logits, draft_logits))
+    for i in range(b):
+        for j in range(g):
+            p, q = (plain.softmax_kept(t[i, j].numpy(), temperature, top_k) for t in (logits, draft_logits))
+            x = int(np.argmax(np.where(q > 1.1 * p, p, -1.0)))               # the target's likeliest among those the draft has too much of
+            assert 0 < p[x] < q[x]
+            drafts[i, j] = x
+            draws[i, j] = p[x] / q[x] * (1 + (-1e-9 if j < i % (g + 1) else 1e-9))
+    _, kept = ops.verify_drafts(logits.cuda(), draft_logits.cuda(), drafts.cuda(), draws.cuda(), temperature, top_k)
+    assert kept.tolist() == [i % (g + 1) for i in range(b)]
+
+
+@gpu
 @pytest.mark.parametrize("temperature", [1e-37, 1e-42, 5e-324])
 @pytest.mark.parametrize("top_k", [0, 40, 700])
 def test_verification_at_the_lowest_temperatures(temperature, top_k):
