@@ -8,7 +8,7 @@
 // whole.  The tokens are then distributed as p's.  Greedy: a draft is taken while it is its row's first maximum.
 //
 // Where nothing is left of max(p - q, 0) (p and q equal) the token comes from p; where p has no mass either (a row without a
-// finite logit) it is the row's first maximum.
+// finite logit, or one with a NaN) it is the row's first maximum, a NaN being larger than every number.
 //
 // Two launches.  The first reads every row once.  Without a top_k: its maximum and its sum of exp((l - max) / T), which are bound
 // by the reading.  With one: the k largest logits, as a list (verify_top_kernel).  Greedy: the first maximum.  The second
@@ -30,15 +30,18 @@ namespace cg = cooperative_groups;
 
 namespace mu {
 
-__device__ __forceinline__ unsigned int order_key(float v) {          // orders as the floats do
-    const unsigned int b = __float_as_uint(v + 0.0f);                 // (-0 is 0)
-    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+// Orders as the floats do, -0 and 0 the same; a NaN without a sign is above them all, one with a sign below.  (By whole numbers: of
+// v + 0.0f the compiler takes a NaN's sign as it likes.)
+__device__ __forceinline__ unsigned int order_key(float v) {
+    const unsigned int b = __float_as_uint(v);
+    return 0x80000000u + ((b & 0x80000000u) ? 0u - (b & 0x7FFFFFFFu) : b);
 }
 __device__ __forceinline__ float key_value(unsigned int k) {
-    return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+    return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : 0x80000000u | (0x80000000u - k));
 }
-__device__ __forceinline__ unsigned long long best_of(float v, int i) {       // a larger logit wins, among equals the lower index
-    return ((unsigned long long)order_key(v) << 32) | (0xFFFFFFFFu - (unsigned int)i);
+// A larger logit wins, any NaN against every number; among equals the lower index.
+__device__ __forceinline__ unsigned long long best_of(float v, int i) {
+    return ((unsigned long long)(v != v ? 0xFFFFFFFFu : order_key(v)) << 32) | (0xFFFFFFFFu - (unsigned int)i);
 }
 __device__ __forceinline__ unsigned long long larger(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
 __device__ __forceinline__ unsigned long long warp_best(unsigned long long v) {
@@ -145,13 +148,18 @@ verify_best_kernel(const VerifyRows rows, int parts, VerifyPart* __restrict__ ou
     unsigned long long best = 0;
     float high = -INFINITY;
     int at = -1;                                                      // the thread's first maximum among the pieces, which come in rising order
+    bool nan = false;
     for_share<VS_THREADS>(row, begin, end, [&](const float (&l)[16], int i) {
         if (at < 0) { high = l[0]; at = i; }
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
+        for (int e = 0; e < 16; ++e) {
             if (l[e] > high) { high = l[e]; at = i + (e / 4) * 4 * VS_THREADS + e % 4; }
+            nan |= l[e] != l[e];
+        }
     }, [&](float l, int i) { best = best_of(l, i); });
     if (at >= 0) best = larger(best, best_of(high, at));
+    if (__syncthreads_or(nan))                                        // comparisons pass NaNs by: entry by entry
+        for (int i = begin + (int)threadIdx.x; i < end; i += VS_THREADS) best = larger(best, best_of(row[i], i));
     best = warp_best(best);
     if ((threadIdx.x & 31) == 0) best_s[threadIdx.x >> 5] = best;
     __syncthreads();
@@ -229,13 +237,16 @@ constexpr int VK_CANDIDATES = 2048;
 constexpr int VERIFY_LIST = 512;          // the largest top_k whose kept logits are handed on as a list
 constexpr int VK_MERGE = 2048;            // entries that a cluster's first block ranks
 
+constexpr unsigned int LOWEST_KEY = 0x00800000u;       // of -inf: no number has a smaller one
+
 // The threshold of the top_k largest by counts over the whole row or share, a bit at a time: each(f) calls f(logit, index) for a
-// thread's logits, `total` is a shared word.  threshold and last as VerifyPart has them.
+// thread's logits, `total` is a shared word.  threshold and last as VerifyPart has them; NaNs are not counted, and where there are
+// fewer numbers than top_k the threshold is 0 (everything is kept).  The counts compare floats: one operation a logit.
 template <typename Each>
 __device__ __forceinline__ void cut_by_counts(Each each, int top_k, int vocab, int* total, unsigned int& threshold, int& last) {
     auto count_where = [&](auto test) {                    // the same for every thread
         int n = 0;
-        each([&](float l, int i) { n += test(order_key(l), i); });
+        each([&](float l, int i) { n += test(l, i); });
         __syncthreads();
         if (threadIdx.x == 0) *total = 0;
         __syncthreads();
@@ -246,16 +257,20 @@ __device__ __forceinline__ void cut_by_counts(Each each, int top_k, int vocab, i
     threshold = 0;
     for (unsigned int bit = 0x80000000u; bit; bit >>= 1) {
         const unsigned int trial = threshold | bit;
-        if (count_where([&](unsigned int k, int) { return k >= trial; }) >= top_k) threshold = trial;
+        const float t = key_value(trial);                  // (above inf's key a NaN: nothing reaches it)
+        if (trial >= LOWEST_KEY && count_where([&](float l, int) { return l >= t; }) >= top_k) threshold = trial;
     }
-    const unsigned int t = threshold;
-    const int room = top_k - count_where([&](unsigned int k, int) { return k > t; });          // of those equal to it, at least one
-    int cut = 0;                                           // the largest index below which fewer than `room` are equal to it
-    for (int bit = 1 << 30; bit; bit >>= 1) {
-        const int trial = cut + bit;
-        if (trial > cut && trial <= vocab && count_where([&](unsigned int k, int i) { return k == t && i < trial; }) < room) cut = trial;
+    last = vocab;
+    if (threshold >= LOWEST_KEY) {
+        const float t = key_value(threshold);
+        const int room = top_k - count_where([&](float l, int) { return l > t; });          // of those equal to it, at least one
+        int cut = 0;                                       // the largest index below which fewer than `room` are equal to it
+        for (int bit = 1 << 30; bit; bit >>= 1) {
+            const int trial = cut + bit;
+            if (trial > cut && trial <= vocab && count_where([&](float l, int i) { return l == t && i < trial; }) < room) cut = trial;
+        }
+        last = cut;
     }
-    last = cut;
     __syncthreads();
 }
 
@@ -351,17 +366,22 @@ verify_top_kernel(const VerifyRows rows, const int* __restrict__ drafts, double 
         unsigned int t;
         int last;
         cut_by_counts(each, top_k, rows.vocab, &total, t, last);
-        if (tid == 0) count = 0;
+        if (tid == 0) { count = 0; total = rows.vocab; }
         __syncthreads();
+        const float least_kept = key_value(t);
         each([&](float l, int i) {
-            const unsigned int k = order_key(l);
-            if (k > t || (k == t && i <= last)) {
+            if (l != l) atomicMin(&total, i);              // the first NaN
+            // (fewer numbers than top_k: the first top_k entries, the first NaN among them)
+            if (t >= LOWEST_KEY ? l > least_kept || (l == least_kept && i <= last) : i - begin < top_k) {
                 const int at = atomicAdd(&count, 1);
                 if (at < VK_CANDIDATES) list[at] = best_of(l, i);        // (exactly top_k of them)
             }
         });
         __syncthreads();
-        rank_all(list, top_k);
+        const bool with_nan = t >= LOWEST_KEY && total < rows.vocab;
+        if (with_nan && tid == 0) list[top_k] = best_of(__uint_as_float(0x7FFFFFFFu), total);
+        __syncthreads();
+        rank_all(list, top_k + (with_nan ? 1 : 0));
     }
     if (blocks > 1) {
         cluster.sync();

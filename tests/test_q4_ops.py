@@ -475,6 +475,32 @@ def test_verification_with_masked_logits():
 
 
 @gpu
+@pytest.mark.parametrize("vocab", [300, 5000, 50257])
+def test_verification_of_rows_without_a_distribution(vocab):
+    """Rows with a NaN somewhere, with an infinity, masked whole: the token is the row's first maximum, a NaN above every number, as the
+    sampler's ``argmax`` has it, wherever it lies; rows beside them are as ever."""
+    rng = np.random.default_rng(vocab)
+    rows = normal((60, vocab), 5)
+    for i in range(40):
+        for at in rng.integers(0, vocab, size=1 + i % 3):
+            rows[i, at] = float("nan")
+    rows[36:40] = torch.where(rows[36:40].isnan(), rows[36:40], torch.tensor(1.25))          # more equal ones than a block ranks
+    rows[39, 5:] = float("nan")
+    rows[40:44, 7], rows[44:48] = float("inf"), -float("inf")
+    rows = rows.cuda()
+    want = ops.argmax(rows)
+    assert torch.equal(want.long(), rows.argmax(dim=1))
+    rows.view(torch.int32)[20:40][rows[20:40].isnan()] = -4194304            # a NaN with its sign set
+    drafts = torch.zeros(60, 0, dtype=torch.int32, device="cuda")
+    draws = torch.rand((60, 1), dtype=torch.float64).cuda()
+    for temperature, top_k in ((0.0, 0), (1.0, 0), (0.7, 20), (0.7, 600)):
+        tokens, kept = ops.verify_drafts(rows[:, None], None, drafts, draws, temperature, top_k)
+        upto = 48 if temperature > 0 else 60
+        assert torch.equal(tokens[:upto, 0], want[:upto]) and (kept == 0).all()
+    check_verify(rows[48:, None].cpu(), torch.zeros(12, 0, vocab), drafts[48:].cpu(), draws[48:].cpu(), 0.7, 20)
+
+
+@gpu
 def test_verification_where_the_draft_is_the_target():
     """p and q equal: every draft is taken; where a draft that is not the row's own is refused, the token comes from p."""
     logits, _, drafts, draws = verify_case(30, 4, 500, 7)
