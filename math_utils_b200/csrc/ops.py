@@ -204,7 +204,7 @@ _SIGNATURES = {
 
 # Arguments that go to the library as one record (LinearQ4Args in q4_linear.cu, NormQ8Args in q8_rows.cu, VerifyArgs in verify.cu):
 # twenty arguments one by one cost 1.9 us of the host, packed 0.4.
-_LINEAR_Q4_ARGS = struct.Struct("13P3q7if")
+_LINEAR_Q4_ARGS = struct.Struct("13P3q7ifi4x")
 _NORM_Q8_ARGS = struct.Struct("8P3q3f3i")
 _VERIFY_ARGS = struct.Struct("8P4qd6i")
 
@@ -1738,6 +1738,12 @@ class Q4Weight(NamedTuple):
     scales: torch.Tensor
 
 
+class FixedQ4Weight(Q4Weight):
+    """A ``Q4Weight`` that no work under way on any stream writes, and the same of every bias and norm's gamma and beta that goes with
+    it (a loaded model's): ``linear_q4`` then fetches them before the launches in front of it on its stream have ended."""
+    __slots__ = ()
+
+
 class Q8Rows(NamedTuple):
     """Rows [m, k] in 8 bits with a power-of-two scale for every 32 entries: ``codes`` float8_e4m3fn [m, kp], ``scales``
     laid out as ``Q4Weight``'s (rows past m have scales that nothing uses, but columns from k on have codes of zero)."""
@@ -1863,7 +1869,8 @@ def linear_q4(x, weight: Q4Weight, bias: Optional[torch.Tensor] = None, act: Opt
     ``out`` bfloat16 (the default) or float32; ``bias`` float32 [n], ``residual`` float32 [m, n], which may be ``out``.
     A row that holds an infinity or NaN gives NaN.  ``way``: 0, or which kernel runs: 1 + b the one for few rows (up to
     64) with b blocks a tile (0: the library chooses), -64, -128, -192 or -256 the one for many with tiles that
-    wide."""
+    wide.  Everything is read after the work in front of the call on its stream, weights, bias, gamma and beta that go with a
+    ``FixedQ4Weight`` apart."""
     norm = None
     if type(x) is NormedInput:
         # the LayerNorms of a few rows are made by the product's own blocks
@@ -1928,7 +1935,7 @@ def linear_q4(x, weight: Q4Weight, bias: Optional[torch.Tensor] = None, act: Opt
         0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), out.data_ptr(),
         0 if room is None else room.data_ptr(), status_word(codes.device).data_ptr(), _stream(), 0 if norm is None else norm.gamma.data_ptr(),
         0 if norm is None or norm.beta is None else norm.beta.data_ptr(), 0 if norm is None or norm.rows is None else norm.rows.data_ptr(),
-        ldx, out.stride(0), ldr, m, n, k, kp, code, out_bf16, way, 0.0 if norm is None else norm.eps)), ("linear_q4({}x{}x{})", m, n, k), launches=1 if room is None else 2)
+        ldx, out.stride(0), ldr, m, n, k, kp, code, out_bf16, way, 0.0 if norm is None else norm.eps, type(weight) is FixedQ4Weight)), ("linear_q4({}x{}x{})", m, n, k), launches=1 if room is None else 2)
     return out
 
 

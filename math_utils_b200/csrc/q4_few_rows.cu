@@ -121,7 +121,7 @@ template <int NB, int MODE, typename TC>
 __global__ void __launch_bounds__(qf_cuts(MODE) ? QF_THREADS_CUT : QF_THREADS)
 q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const unsigned char* __restrict__ w_scales, const QfRows rows,
                    const float* __restrict__ bias, const float* residual, TC* C, int M, int N, int kb_all, long long ldc,
-                   long long ldr, int act, int* status, int splits, int stages) {
+                   long long ldr, int act, int* status, int splits, int stages, int fixed) {
     constexpr int PIECES = MODE == QF_EIGHT ? 1 : 2;
     constexpr int NX = PIECES * NB;                       // rows as the instruction sees them: the pieces one behind the other
     constexpr uint32_t X_PIECE = NB * QF_BK, STAGE = QF_W_BYTES + PIECES * X_PIECE;
@@ -159,6 +159,7 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                      ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (!fixed) pdl_wait();                               // weights, bias, gamma and beta may be the work of earlier kernels
     if (threadIdx.x >= 64 && threadIdx.x < 192) {
         const int n = n0 + (int)threadIdx.x - 64;
         bias_s[threadIdx.x - 64] = (bias && n < N) ? bias[n] : 0.0f;
@@ -189,7 +190,7 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
                 }
                 if (++kb == my_kb) kb = 0;
             };
-            if (!weights) pdl_wait();                     // (weights are written by no kernel)
+            if (!weights) pdl_wait();                     // (the weights: above, unless they are fixed)
             const int first = my_kb < stages ? my_kb : stages;
             for (int i = 0; i < first; ++i) load(i);
             int issued = first, s = 0;
@@ -244,7 +245,7 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             constexpr int PAIRS = NB / 4;                          // of rows, a warp
             const int turn = (warp - 2) & 3, pair0 = (warp - 2) >> 2;
             const int half = lane >> 4, c8 = lane & 15;
-            // QF_NORMED: gamma and beta of this block's share of k to shared memory (parameters: before the wait), then a row's mean and
+            // QF_NORMED: gamma and beta of this block's share of k to shared memory (before the wait where they are fixed), then a row's mean and
             // inverse deviation by a warp each
             float* gamma_s = reinterpret_cast<float*>(scale_smem + (size_t)stages * SCALE_STAGE);
             float* beta_s = gamma_s + my_kb * QF_BK;
@@ -482,7 +483,7 @@ q4_few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 template <int NB, int MODE, typename TC>
 static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const unsigned char* w_scales,
                       const QfRows& rows, const float* bias, const float* residual, TC* C, int M, int N, int kb_all, long long ldc,
-                      long long ldr, int act, int* status, int splits, int stages, size_t smem, cudaStream_t s) {
+                      long long ldr, int act, int* status, int splits, int stages, int fixed, size_t smem, cudaStream_t s) {
     auto kernel = q4_few_rows_kernel<NB, MODE, TC>;
     if (!allow_shared(reinterpret_cast<const void*>(kernel), 224 * 1024)) return MU_ERR_LAUNCH;
     const int tiles = (N + QF_BN - 1) / QF_BN;
@@ -508,7 +509,7 @@ static int launch_few(const CUtensorMap& map_w, const CUtensorMap& map_x, const 
     cfg.attrs = attr;
     cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, w_scales, rows, bias, residual, C, M, N, kb_all, ldc, ldr, act,
-                              status, splits, stages) == cudaSuccess ? MU_OK : MU_ERR_LAUNCH;
+                              status, splits, stages, fixed) == cudaSuccess ? MU_OK : MU_ERR_LAUNCH;
 }
 
 static bool tensor_map_codes(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long rows, int kp, long long row_bytes,
@@ -569,7 +570,7 @@ int q4_few_rows_tile(int M, bool cut_here) { return cut_here ? 8 : M <= 16 ? 16 
 // (scales null) bfloat16 x [M, K] (ldx), M <= 8; or (norm not null) the LayerNorms of float32 x [.][K] (ldx), M <= 8.  splits: blocks that share a tile and cut K (up to 8; 0: chosen here).
 int launch_q4_few_rows(const void* x, const void* x_scales, bool two_pieces, long long ldx, int K, const void* w, const void* w_scales,
                        const float* bias, const float* residual, void* C, int M, int N, int kp, long long ldc, long long ldr, int act,
-                       int out_bf16, int splits, const RowNorm* norm, int* status, void* stream) {
+                       int out_bf16, int splits, const RowNorm* norm, int fixed, int* status, void* stream) {
     const int mode = norm ? QF_NORMED : !x_scales ? QF_SIXTEEN : two_pieces ? QF_PIECES : QF_EIGHT;
     if (M > (qf_cuts(mode) ? QF_MAX_CUT : 64)) return MU_ERR_UNSUPPORTED_SIZE;
     if (splits < 0 || splits > QF_MAX_SPLIT) return MU_ERR_BAD_ARGUMENT;
@@ -613,9 +614,9 @@ int launch_q4_few_rows(const void* x, const void* x_scales, bool two_pieces, lon
     cudaStream_t s = (cudaStream_t)stream;
 #define MU_FEW(NB, MODE)                                                                                                            \
     (out_bf16 ? launch_few<NB, MODE, __nv_bfloat16>(map_w, map_x, (const unsigned char*)w_scales, rows, bias, residual, \
-                                                        (__nv_bfloat16*)C, M, N, kb_all, ldc, ldr, act, status, splits, stages, smem, s) \
+                                                        (__nv_bfloat16*)C, M, N, kb_all, ldc, ldr, act, status, splits, stages, fixed, smem, s) \
               : launch_few<NB, MODE, float>(map_w, map_x, (const unsigned char*)w_scales, rows, bias, residual, (float*)C, \
-                                                M, N, kb_all, ldc, ldr, act, status, splits, stages, smem, s))
+                                                M, N, kb_all, ldc, ldr, act, status, splits, stages, fixed, smem, s))
 #define MU_FEW_BOTH(NB) (mode == QF_PIECES ? MU_FEW(NB, QF_PIECES) : MU_FEW(NB, QF_EIGHT))
     if (mode == QF_NORMED) return MU_FEW(8, QF_NORMED);
     if (mode == QF_SIXTEEN) return MU_FEW(8, QF_SIXTEEN);

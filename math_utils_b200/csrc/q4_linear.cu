@@ -6,10 +6,10 @@ namespace mu {
 int q4_few_rows_tile(int M, bool cut_here);
 int launch_q4_few_rows(const void* x, const void* x_scales, bool two_pieces, long long ldx, int K, const void* w, const void* w_scales,
                        const float* bias, const float* residual, void* C, int M, int N, int kp, long long ldc, long long ldr, int act,
-                       int out_bf16, int splits, const RowNorm* norm, int* status, void* stream);
+                       int out_bf16, int splits, const RowNorm* norm, int fixed, int* status, void* stream);
 int launch_q4_prompt(const void* x0, const void* x0_scales, const void* x1, const void* x1_scales, const void* w, const void* w_scales,
                      const float* bias, const float* residual, void* C, int M, int N, int kp, long long ldc, long long ldr, int act,
-                     int out_bf16, int bn, int* status, void* stream);
+                     int out_bf16, int bn, int fixed, int* status, void* stream);
 int launch_quantize_q8(const void* x, long long ldx, int is_bf16, int m, int k, int kp, int behind, void* codes, void* scales, void* stream);
 
 // Up to 32 rows go to the kernel with the weights as the wide operand; up to 64 where that kernel can cut a long k and the other
@@ -35,6 +35,8 @@ struct LinearQ4Args {
     long long ldx, ldo, ldr;
     int m, n, k, kp, act, out_bf16, way; // way 0: the kernel is chosen here; tests: 1 + blocks a tile, or -(columns of a tile)
     float eps;
+    int fixed;                           // weights, exponents, bias, gamma and beta are written by no work that may still be under way on any
+                                         // stream: they are fetched before the launches in front of this one have ended
 };
 
 constexpr int Q4_CUT_INSIDE = 8;         // bfloat16 rows that the few-rows kernel cuts itself
@@ -74,7 +76,7 @@ MU_EXPORT int mu_linear_q4(const LinearQ4Args* p) {
     }
     if (few)
         return mu::launch_q4_few_rows(x, scales, cut, ldx, a.k, a.w, a.w_scales, a.bias, a.residual, a.out, a.m, a.n, a.kp, ldo, ldr, a.act,
-                                      a.out_bf16, a.way > 0 ? a.way - 1 : 0, a.gamma ? &norm : nullptr, a.status, a.stream);
+                                      a.out_bf16, a.way > 0 ? a.way - 1 : 0, a.gamma ? &norm : nullptr, a.fixed, a.status, a.stream);
     return mu::launch_q4_prompt(x, scales, x1, scales1, a.w, a.w_scales, a.bias, a.residual, a.out, a.m, a.n, a.kp, ldo, ldr, a.act, a.out_bf16,
-                                -a.way, a.status, a.stream);
+                                -a.way, a.fixed, a.status, a.stream);
 }

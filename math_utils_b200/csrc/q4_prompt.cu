@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(QP_THREADS, 1)
 q4_prompt_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_constant__ CUtensorMap map_x1,
                  const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_c, const QpScales scales,
                  const float* __restrict__ bias, const float* residual, TC* C, int M, int N, int kb_all, long long ldc, long long ldr,
-                 int act, int* status, int bulk_out) {
+                 int act, int* status, int bulk_out, int fixed) {
     extern __shared__ unsigned char qp_raw[];
     typedef QpSmem<BN, PIECES, STAGES> Smem;
     Smem& sm = *reinterpret_cast<Smem*>(((uintptr_t)qp_raw + 1023) & ~(uintptr_t)1023);
@@ -67,7 +67,7 @@ q4_prompt_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_consta
     if (warp == 0 || warp == 10) {
         if (lane == 0) {
             const bool rows = warp == 0;
-            if (rows) pdl_wait();                             // (weights are written by no kernel)
+            if (rows || !fixed) pdl_wait();                   // (fixed weights are written by no kernel)
             long long issued = 0;
             int s = 0;
             uint32_t phase = 1;                               // an empty ring's stages count as given back
@@ -213,7 +213,7 @@ q4_prompt_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_consta
 
 template <int BN, int PIECES, int STAGES, typename TC>
 static int launch_prompt(const void* x0, const void* x1, const void* w, const QpScales& scales, const float* bias, const float* residual,
-                         TC* C, int M, int N, int kp, long long ldc, long long ldr, int act, int* status, cudaStream_t s) {
+                         TC* C, int M, int N, int kp, long long ldc, long long ldr, int act, int fixed, int* status, cudaStream_t s) {
     CUtensorMap map_x0, map_x1, map_w, map_c;
     if (!tensor_map_q8(&map_x0, x0, M, kp, TC_BM) || !tensor_map_q4(&map_w, w, N, kp, BN)) return MU_ERR_LAUNCH;
     map_x1 = map_x0;
@@ -234,7 +234,7 @@ static int launch_prompt(const void* x0, const void* x1, const void* w, const Qp
     const long long tiles = (long long)((N + BN - 1) / BN) * ((M + TC_BM - 1) / TC_BM);
     if (tiles > 2147483647ll - sms) return MU_ERR_UNSUPPORTED_SIZE;
     return launch_pdl(kernel, dim3((unsigned)(tiles < sms ? tiles : sms)), dim3(QP_THREADS), smem, s, 1, map_x0, map_x1, map_w, map_c, scales,
-                      bias, residual, C, M, N, kp / QP_BK, ldc, ldr, act, status, bulk_out);
+                      bias, residual, C, M, N, kp / QP_BK, ldc, ldr, act, status, bulk_out, fixed);
 }
 
 // The columns of a tile, by the cycles of the waves that its tiles make: a stage of 128 of k takes its products (2 cycles a column
@@ -261,15 +261,15 @@ static int choose_columns(int M, int N, int kb, int pieces, int sms) {
 // chosen here).
 int launch_q4_prompt(const void* x0, const void* x0_scales, const void* x1, const void* x1_scales, const void* w, const void* w_scales,
                            const float* bias, const float* residual, void* C, int M, int N, int kp, long long ldc, long long ldr, int act,
-                           int out_bf16, int bn, int* status, void* stream) {
+                           int out_bf16, int bn, int fixed, int* status, void* stream) {
     const QpScales scales = {{(const unsigned char*)x0_scales, (const unsigned char*)x1_scales}, (const unsigned char*)w_scales};
     const int sms = sm_count();
     if (sms <= 0) return MU_ERR_LAUNCH;
     if (bn == 0) bn = choose_columns(M, N, kp / QP_BK, x1 ? 2 : 1, sms);
     cudaStream_t s = (cudaStream_t)stream;
 #define MU_QP(BN, P, ST)                                                                                                            \
-    (out_bf16 ? launch_prompt<BN, P, ST, __nv_bfloat16>(x0, x1, w, scales, bias, residual, (__nv_bfloat16*)C, M, N, kp, ldc, ldr, act, status, s) \
-              : launch_prompt<BN, P, ST, float>(x0, x1, w, scales, bias, residual, (float*)C, M, N, kp, ldc, ldr, act, status, s))
+    (out_bf16 ? launch_prompt<BN, P, ST, __nv_bfloat16>(x0, x1, w, scales, bias, residual, (__nv_bfloat16*)C, M, N, kp, ldc, ldr, act, fixed, status, s) \
+              : launch_prompt<BN, P, ST, float>(x0, x1, w, scales, bias, residual, (float*)C, M, N, kp, ldc, ldr, act, fixed, status, s))
     if (bn == 256) return x1 ? MU_QP(256, 2, 2) : MU_QP(256, 1, 3);
     if (bn == 192) return x1 ? MU_QP(192, 2, 3) : MU_QP(192, 1, 4);
     if (bn == 128) return x1 ? MU_QP(128, 2, 3) : MU_QP(128, 1, 5);

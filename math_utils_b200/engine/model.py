@@ -39,6 +39,8 @@ class DecoderModel:
         self._workspace: dict = {}
         self.weight_bytes = sum(t.numel() * t.element_size() for t in tensors.values()) - getattr(runtime, "saved_bytes", 0)
         self.graph_safe = all(getattr(p, "graph_safe", True) for p in self.assembly.parts())
+        if runtime.device.type == "cuda":
+            torch.cuda.synchronize(runtime.device)      # steps, on whatever stream, fetch weights before they wait for what is in front of them
 
     # ---------------------------------------------------------------- loading
     @classmethod

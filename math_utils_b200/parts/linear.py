@@ -22,7 +22,8 @@ import torch
 class Linear:
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor], runtime, keep: bool = False):
         self.quantised = getattr(runtime, "weight_bits", 16) == 4 and not keep
-        self.weight = runtime.ops.quantize_q4(weight) if self.quantised else weight     # [out, in], compute dtype unless in 4 bits
+        # [out, in], compute dtype unless in 4 bits
+        self.weight = runtime.ops.FixedQ4Weight(*runtime.ops.quantize_q4(weight)) if self.quantised else weight
         if self.quantised:
             runtime.saved_bytes += (weight.numel() * weight.element_size()
                                     - sum(t.numel() * t.element_size() for t in self.weight))

@@ -606,6 +606,67 @@ def test_calls_on_two_streams_at_once_and_in_graphs():
     ops.check_status()
 
 
+def test_only_fixed_weights_are_fetched_early(monkeypatch):
+    """What the kernels are told: a weight is fetched ahead of the work in front of the call where its type says that nothing writes
+    it any more, as a loaded model's does, and not otherwise."""
+    from math_utils_b200.parts.linear import Linear
+    records = []
+
+    class Library:
+        @staticmethod
+        def mu_linear_q4(record):
+            records.append(ops._LINEAR_Q4_ARGS.unpack(record))
+            return 0
+
+    monkeypatch.setattr(ops, "library", Library)
+    monkeypatch.setattr(ops, "_on_current_device", lambda *t: None)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "status_word", lambda device: torch.zeros(1, dtype=torch.int32))
+    w = fake_weight(200, 300)
+    monkeypatch.setattr(ops, "quantize_q4", lambda given: w)
+    for x in (torch.zeros(4, 300, dtype=torch.bfloat16), torch.zeros(40, 300, dtype=torch.bfloat16), fake_rows(4, 300)):
+        ops.linear_q4(x, w)
+        ops.linear_q4(x, ops.FixedQ4Weight(*w))
+    assert [r[-1] for r in records] == [0, 1] * 3
+
+    class Runtime:
+        weight_bits, row_bits, saved_bytes = 4, 16, 0
+    Runtime.ops = ops
+    Linear(torch.zeros(200, 300, dtype=torch.bfloat16), None, Runtime)(torch.zeros(4, 300, dtype=torch.bfloat16))
+    assert records[-1][-1] == 1
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 8, 20, 200])
+def test_products_of_weights_written_right_before(m):
+    """Codes, exponents and bias that the kernel in front of the call writes, eagerly and in a recorded graph, and whatever ran in front of
+    that (the product before lets its successor in early)."""
+    x = normal((m, 1300), 1).bfloat16().cuda()
+    sets = [(ops.quantize_q4(normal((700, 1300), s, 0.05).cuda()), normal((700,), s + 50).cuda()) for s in (2, 3)]
+    want = [ops.linear_q4(x, w, bias=b, out_dtype=torch.float32) for w, b in sets]
+    held, bias = Q4Weight(*(t.clone() for t in sets[0][0])), sets[0][1].clone()
+
+    def write(i):                                           # kernels, not copies: a copy would order everything after it
+        codes, scales = (t.view(torch.uint8) for t in sets[i][0])
+        torch.bitwise_or(codes, 0, out=held.codes)
+        torch.bitwise_or(scales, 0, out=held.scales.view(torch.uint8))
+        torch.add(sets[i][1], 0.0, out=bias)
+        return ops.linear_q4(x, held, bias=bias, out_dtype=torch.float32)
+
+    for turn in range(20):
+        assert torch.equal(write(turn % 2), want[turn % 2])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = [write(turn % 2) for turn in range(10)]
+    for _ in range(5):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[turn % 2]) for turn, g in enumerate(got))
+    ops.check_status()
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def fake_weight(n, k):
     kp = plain.padded(k)
