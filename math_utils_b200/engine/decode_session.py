@@ -323,15 +323,17 @@ class DecodeSession:
 _SESSIONS_KEPT = 6
 
 
-def session_for(model, cache, params: SamplingParams, n: int, pipelined: bool = True) -> DecodeSession:
+def session_for(model, cache, params: SamplingParams, n: int, pipelined: bool = True,
+                kv_bound: Optional[int] = None) -> DecodeSession:
     """A session of ``n`` sequences for this model, cache and sampling rule; the
-    last few are kept so that batch after batch replays the same graphs."""
+    last few are kept so that batch after batch replays the same graphs.
+    ``kv_bound``: positions that no sequence goes past, the model's most if not given."""
     kept = model.__dict__.setdefault("_decode_sessions", {})
-    key = (id(cache), n, params, pipelined)
+    kv_bound = model.max_positions if kv_bound is None else kv_bound
+    key = (id(cache), n, params, pipelined, kv_bound)
     session = kept.pop(key, None)
     if session is None or session.cache is not cache:
-        session = DecodeSession(model, cache, [0] * n, params, [0] * n, kv_bound=model.max_positions,
-                                pipelined=pipelined)
+        session = DecodeSession(model, cache, [0] * n, params, [0] * n, kv_bound=kv_bound, pipelined=pipelined)
     kept[key] = session                                  # most recently used last
     while len(kept) > _SESSIONS_KEPT:
         kept.pop(next(iter(kept)))

@@ -7,8 +7,10 @@ the drafts) as ONE step with the logits of every position wanted, which costs it
 target's own (greedy: are the target's own).  Both caches are then cut back to what stood.
 
 Any two models over one vocabulary will do; the natural draft is the same weights in 4 bits.  Caches that cannot be cut
-back (windows, fixed-size state) are refused.  Random numbers: a request's draws depend on its seed and index alone; the
-draft's samples and the verification use streams of their own.
+back (windows, fixed-size state) are refused.  Random numbers: a request's draws, and which of them meets which of its
+tokens, depend on its seed and index alone, whatever else its batch holds: every round takes ``drafts`` + 1 numbers of the
+request's stream and of the draft's, also where the context's end leaves fewer drafts.  The draft's samples and the
+verification use streams of their own.
 """
 from __future__ import annotations
 
@@ -51,6 +53,7 @@ def run_drafted(model, draft, cache, draft_cache, params: SamplingParams, states
     ``kept_slots``: a (slot, draft slot) pair for each request, taken by the caller; they are not given back, and at the end
     hold exactly what was fed and emitted.  ``counts``: receives ``rounds``, ``drafted`` and ``kept``."""
     check_draftable(model, draft, cache, draft_cache)
+    context = min(context, model.max_positions, draft.max_positions)
     ops, device = model.runtime.ops, model.runtime.device
     draft_params = SamplingParams(params.temperature, params.top_k, params.seed ^ _DRAFT_STREAM)
     tally = counts if counts is not None else {}
@@ -83,32 +86,38 @@ def run_drafted(model, draft, cache, draft_cache, params: SamplingParams, states
             import time
             first_sample.append(time.perf_counter())
         check_kernels(model)
-        used = {k: 1 for k in live}                            # draws of each request's own stream
-        drawn = 0                                              # draws of the draft's streams, the same for all
         for k in list(live):
             if not take_token(states[k], last[k], stop_ids, max_tokens, context):
                 live.remove(k)
                 leave(k)
+        drawn = 0                   # numbers that the rounds so far have taken of each request's streams
         while live:
-            starts = [cache.length(slots[k][0]) for k in live]
-            g = room_for_drafts(model, draft, starts, drafts, context)
-            n = len(live)
+            starts = {k: cache.length(slots[k][0]) for k in live}
+            room = {k: room_for_drafts(model, draft, [starts[k]], drafts, context) for k in live}
+            g, n = max(room.values()), len(live)
             ids, qs = _draft(draft, draft_cache, draft_params, [slots[k][1] for k in live], [states[k].index for k in live],
-                             [last[k] for k in live], g, drawn)
-            drawn += g + 1
-            rows = ids.cpu().tolist() if g else [[] for _ in live]
-            logits = model.step(cache, [StepEntry(slots[k][0], [last[k]] + r, range(g + 1)) for k, r in zip(live, rows)])
-            draws = np.stack([uniform_draws(params.seed, states[k].index, used[k], g + 1) for k in live])
+                             [last[k] for k in live], [room[k] for k in live], g, drawn, context)
+            rows = [row[:room[k]] for k, row in zip(live, ids.cpu().tolist())] if g else [[] for _ in live]
+            logits = model.step(cache, [StepEntry(slots[k][0], [last[k]] + r, range(len(r) + 1)) for k, r in zip(live, rows)])
+            if min(room.values()) < g:                             # near the context's end: every sequence in g + 1 rows, the drafts end at a -1
+                places = torch.arange(g, device=device)
+                ids = ids.masked_fill(places >= torch.tensor([room[k] for k in live], device=device)[:, None], -1)
+                wide = logits.new_zeros((n * (g + 1), logits.shape[1]))
+                wide[torch.tensor([i * (g + 1) + j for i, r in enumerate(rows) for j in range(len(r) + 1)], device=device)] = logits
+                logits = wide
+            # the token behind the drafts taken comes from the round's last number, however many drafts there were
+            draws = np.stack([uniform_draws(params.seed, states[k].index, 1 + drawn, drafts + 1) for k in live])
+            draws = np.concatenate([draws[:, :g], draws[:, drafts:]], axis=1)
             tokens, kept = ops.verify_drafts(logits.view(n, g + 1, -1), qs, ids, torch.from_numpy(draws).to(device),
                                              params.temperature if not params.greedy else 0.0, params.kept)
             answer = torch.cat([tokens, kept[:, None]], dim=1).cpu().tolist()
             check_kernels(model)
+            drawn += drafts + 1
             tally["rounds"] += 1
-            tally["drafted"] += g * n
-            for k, start, row in zip(list(live), starts, answer):
-                stood = row[-1]
+            tally["drafted"] += sum(room.values())
+            for k, row in zip(list(live), answer):
+                start, stood = starts[k], row[-1]
                 tally["kept"] += stood
-                used[k] += g + 1
                 # what both models have been fed and what stands of it: the last token and the drafts kept
                 cache.truncate(slots[k][0], start + 1 + stood)
                 draft_cache.truncate(slots[k][1], start + 1 + stood)
@@ -135,17 +144,21 @@ def run_drafted(model, draft, cache, draft_cache, params: SamplingParams, states
                 draft_cache.release(b)
 
 
-def _draft(draft, cache, params: SamplingParams, slots: Sequence[int], requests: Sequence[int], tokens: Sequence[int], g: int,
-           drawn: int):
+def _draft(draft, cache, params: SamplingParams, slots: Sequence[int], requests: Sequence[int], tokens: Sequence[int],
+           rooms: Sequence[int], g: int, drawn: int, context: int):
     """``g`` tokens drafted behind ``tokens``: (ids int32 [n, g], the logits they were sampled from [n, g, vocab], or None
-    where greedy).  The draft is stepped once more, so that its cache holds the last one too."""
+    where greedy).  The draft is stepped once more, so that its cache holds the last one too.
+
+    ``rooms``: how many of the g each sequence has room for.  The recorded step moves every sequence on g + 1 times, but none past
+    the context's last position, where one without room for more stays: what it writes there is no part of it, since a
+    sequence that fills the context ends without that position."""
     n, device = len(slots), draft.runtime.device
-    session = session_for(draft, cache, params, n, pipelined=False)
+    session = session_for(draft, cache, params, n, pipelined=False, kv_bound=context)
     state = (list(slots), list(requests), drawn)
     if getattr(session, "drafts_for", None) != state:          # (else it is where the round before left it)
         session.rebind(slots, requests, [drawn] * n)
     session.drafts_for = (list(slots), list(requests), drawn + g + 1)
-    starts = [cache.reserve(s, g + 1) for s in slots]
+    starts = [cache.reserve(s, room + 1) for s, room in zip(slots, rooms)]
     session.sync_block_tables()
     session.feed(tokens, starts)
     ids = torch.empty((n, g), dtype=torch.int32, device=device)
@@ -156,8 +169,8 @@ def _draft(draft, cache, params: SamplingParams, slots: Sequence[int], requests:
             ids[:, i] = session.next_tokens
             if qs is not None:
                 qs[:, i] = session.logits
-    for s in slots:
-        cache.commit(s, g + 1)
+    for s, room in zip(slots, rooms):
+        cache.commit(s, room + 1)
     return ids, qs
 
 
