@@ -338,3 +338,10 @@ def session_for(model, cache, params: SamplingParams, n: int, pipelined: bool = 
     while len(kept) > _SESSIONS_KEPT:
         kept.pop(next(iter(kept)))
     return session
+
+
+def drop_sessions(model, cache) -> None:
+    """Lets go of the sessions kept for a cache that is not used any more (each holds the cache)."""
+    kept = model.__dict__.get("_decode_sessions", {})
+    for key in [key for key, session in kept.items() if session.cache is cache]:
+        del kept[key]

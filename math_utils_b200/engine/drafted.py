@@ -22,7 +22,7 @@ import torch
 from ..sampling import Sampler, SamplingParams
 from ..sampling.sampler import uniform_draws
 from .batch import StepEntry
-from .decode_session import session_for
+from .decode_session import drop_sessions, session_for
 from .generate import check_kernels, settle, take_token
 
 _DRAFT_STREAM = 0x5851F42D4C957F2D         # what the draft's seed differs by
@@ -90,13 +90,22 @@ def run_drafted(model, draft, cache, draft_cache, params: SamplingParams, states
             if not take_token(states[k], last[k], stop_ids, max_tokens, context):
                 live.remove(k)
                 leave(k)
+        members = list(live)        # whom the draft's recorded step runs: those that have ended stay until half of them have
         drawn = 0                   # numbers that the rounds so far have taken of each request's streams
         while live:
+            if len(live) * 2 <= len(members):
+                for k in members:
+                    if k not in live:
+                        leave(k)
+                members = list(live)
             starts = {k: cache.length(slots[k][0]) for k in live}
             room = {k: room_for_drafts(model, draft, [starts[k]], drafts, context) for k in live}
             g, n = max(room.values()), len(live)
-            ids, qs = _draft(draft, draft_cache, draft_params, [slots[k][1] for k in live], [states[k].index for k in live],
-                             [last[k] for k in live], [room[k] for k in live], g, drawn, context)
+            ids, qs = _draft(draft, draft_cache, draft_params, [slots[k][1] for k in members], [states[k].index for k in members],
+                             [last[k] for k in members], [room.get(k) for k in members], g, drawn, context)
+            if n < len(members):
+                at = torch.tensor([members.index(k) for k in live], device=device)
+                ids, qs = ids[at], None if qs is None else qs[at]
             rows = [row[:room[k]] for k, row in zip(live, ids.cpu().tolist())] if g else [[] for _ in live]
             logits = model.step(cache, [StepEntry(slots[k][0], [last[k]] + r, range(len(r) + 1)) for k, r in zip(live, rows)])
             if min(room.values()) < g:                             # near the context's end: every sequence in g + 1 rows, the drafts end at a -1
@@ -133,7 +142,6 @@ def run_drafted(model, draft, cache, draft_cache, params: SamplingParams, states
                 last[k] = states[k].produced[-1] if states[k].produced else last[k]
                 if not goes_on:
                     live.remove(k)
-                    leave(k)
         if kept_slots is not None:
             settle(model, cache, states, [pair[0] for pair in kept_slots], context)
             settle(draft, draft_cache, states, [pair[1] for pair in kept_slots], context)
@@ -145,20 +153,23 @@ def run_drafted(model, draft, cache, draft_cache, params: SamplingParams, states
 
 
 def _draft(draft, cache, params: SamplingParams, slots: Sequence[int], requests: Sequence[int], tokens: Sequence[int],
-           rooms: Sequence[int], g: int, drawn: int, context: int):
+           rooms: Sequence[Optional[int]], g: int, drawn: int, context: int):
     """``g`` tokens drafted behind ``tokens``: (ids int32 [n, g], the logits they were sampled from [n, g, vocab], or None
     where greedy).  The draft is stepped once more, so that its cache holds the last one too.
 
-    ``rooms``: how many of the g each sequence has room for.  The recorded step moves every sequence on g + 1 times, but none past
-    the context's last position, where one without room for more stays: what it writes there is no part of it, since a
-    sequence that fills the context ends without that position."""
+    ``rooms``: how many of the g each sequence has room for, None for one that has ended.  The recorded step moves every
+    sequence on g + 1 times, but none past the context's last position, where one without room for more stays: what it writes
+    there is no part of it, since a sequence that fills the context ends without that position.  One that has ended writes
+    behind its end, on pages of its own."""
     n, device = len(slots), draft.runtime.device
     session = session_for(draft, cache, params, n, pipelined=False, kv_bound=context)
     state = (list(slots), list(requests), drawn)
     if getattr(session, "drafts_for", None) != state:          # (else it is where the round before left it)
         session.rebind(slots, requests, [drawn] * n)
     session.drafts_for = (list(slots), list(requests), drawn + g + 1)
-    starts = [cache.reserve(s, room + 1) for s, room in zip(slots, rooms)]
+    starts = [min(cache.length(s), context - 1) for s in slots]
+    for s, start, room in zip(slots, starts, rooms):
+        cache.reserve(s, room + 1 if room is not None else min(start + g + 1, context) - cache.length(s))
     session.sync_block_tables()
     session.feed(tokens, starts)
     ids = torch.empty((n, g), dtype=torch.int32, device=device)
@@ -170,16 +181,26 @@ def _draft(draft, cache, params: SamplingParams, slots: Sequence[int], requests:
             if qs is not None:
                 qs[:, i] = session.logits
     for s, room in zip(slots, rooms):
-        cache.commit(s, room + 1)
+        if room is not None:
+            cache.commit(s, room + 1)
     return ids, qs
+
+
+def cache_room(prompts: Sequence[Sequence[int]], max_tokens: int, drafts: int, context: int, max_batch: int) -> int:
+    """Positions that each of the two caches needs for these requests: a round may run ``drafts`` positions past a request's
+    last."""
+    from ..cache import PAGE_TOKENS
+    from .generate import round_up
+    need = sorted((round_up(min(context, len(p) + max_tokens + drafts), PAGE_TOKENS) for p in prompts), reverse=True)
+    return max(sum(need[:max_batch]), PAGE_TOKENS)
 
 
 def generate_drafted(model, draft, prompts: Sequence[Sequence[int]], max_tokens: int, params: SamplingParams, drafts: int,
                      stop_ids=None, context: Optional[int] = None, max_batch: int = 64, cache=None, draft_cache=None,
                      counts: Optional[dict] = None) -> List[List[int]]:
-    """``generate`` with ``drafts`` tokens drafted a round by ``draft``."""
-    from ..cache import PAGE_TOKENS
-    from .generate import RequestState, plan_batches, round_up
+    """``generate`` with ``drafts`` tokens drafted a round by ``draft``.  ``cache`` and ``draft_cache``: the caller's, who calls
+    again and wants neither them nor the recorded steps made anew; without them they are made here and dropped at the end."""
+    from .generate import RequestState, plan_batches
     if drafts < 1:
         raise ValueError(f"at least one token is drafted a round, got {drafts}")
     context = min(context or model.max_positions, model.max_positions, draft.max_positions)
@@ -189,23 +210,26 @@ def generate_drafted(model, draft, prompts: Sequence[Sequence[int]], max_tokens:
             raise ValueError(f"prompt {i} is empty")
         if len(p) > context:
             raise ValueError(f"prompt {i} has {len(p)} tokens, the context holds {context}")
-    # a round may run `drafts` positions past a request's last
-    need = sorted((round_up(min(context, len(p) + max_tokens + drafts), PAGE_TOKENS) for p in prompts), reverse=True)
-    total = max(sum(need[:max_batch]), PAGE_TOKENS)
+    total = cache_room(prompts, max_tokens, drafts, context, max_batch)
     if cache is None:
         cache = model.new_cache(max_tokens=total, n_slots=max_batch)
-    if draft_cache is None:
+    made = draft_cache is None
+    if made:
         draft_cache = draft.new_cache(max_tokens=total, n_slots=max_batch)
     page = cache.page_tokens
     batches = plan_batches([len(p) for p in prompts], max_tokens + drafts + 1, context, min(max_batch, cache.n_slots, draft_cache.n_slots),
                            min(cache.n_pages, draft_cache.n_pages) * page, page)
     states = [RequestState(i, p) for i, p in enumerate(prompts)]
     sums = {"rounds": 0, "drafted": 0, "kept": 0}
-    for batch in batches:
-        here: dict = {}
-        run_drafted(model, draft, cache, draft_cache, params, [states[i] for i in batch], stop, max_tokens, context, drafts, counts=here)
-        for key in sums:
-            sums[key] += here[key]
+    try:
+        for batch in batches:
+            here: dict = {}
+            run_drafted(model, draft, cache, draft_cache, params, [states[i] for i in batch], stop, max_tokens, context, drafts, counts=here)
+            for key in sums:
+                sums[key] += here[key]
+    finally:
+        if made:
+            drop_sessions(draft, draft_cache)
     if counts is not None:
         counts.update(sums)
     return [s.produced for s in states]

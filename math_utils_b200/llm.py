@@ -46,7 +46,7 @@ class LLM:
         self.current = ""
         self._cache = None
         self._batch_cache = None
-        self._draft_cache = self._draft_slot = None
+        self._draft_cache = self._draft_slot = self._draft_batch_cache = None
         self._slot = None
         self._turns = 0
         self.last: dict = {}            # figures of the last prompt(): tokens in and out, seconds, why it ended
@@ -78,7 +78,7 @@ class LLM:
 
     def unload(self) -> None:
         self.model, self._cache, self._slot, self.current, self._turns = None, None, None, "", 0
-        self._batch_cache = self.draft = self._draft_cache = self._draft_slot = None
+        self._batch_cache = self._draft_batch_cache = self.draft = self._draft_cache = self._draft_slot = None
 
     @property
     def loaded(self) -> bool:
@@ -183,25 +183,34 @@ class LLM:
         max_tokens = self.options.max_tokens if max_tokens is None else max_tokens
         max_batch = max_batch or self.options.max_batch
         if self.draft is not None:
-            from .engine.drafted import generate_drafted
+            from .engine.drafted import cache_room, generate_drafted
+            self._hold_batch_caches(cache_room(prompts, max_tokens, self.options.drafts, self.context, max_batch), len(prompts), max_batch)
             self.draft_counts = {}
             return generate_drafted(self.model, self.draft, prompts, max_tokens, self._params(temperature, top_k, seed),
                                     self.options.drafts, stop_ids=stop_ids, context=self.context, max_batch=max_batch,
-                                    counts=self.draft_counts)
-        # One cache serves call after call (and with it the recorded graphs of its batch sizes); a
-        # call that needs more room than any before gets a larger one.
+                                    cache=self._batch_cache, draft_cache=self._draft_batch_cache, counts=self.draft_counts)
         from .cache import PAGE_TOKENS
         from .engine.generate import most_positions, round_up
         need = sorted((round_up(max(most_positions(len(p), max_tokens, self.context), 1), PAGE_TOKENS)
                        for p in prompts), reverse=True)
-        tokens = max(sum(need[:max_batch]), PAGE_TOKENS)
-        held = self._batch_cache
-        if held is None or held.n_pages * held.page_tokens < tokens or held.n_slots < min(max_batch, len(prompts)):
-            self._batch_cache = None
-            self.model.__dict__.pop("_decode_sessions", None)
-            held = self._batch_cache = self.model.new_cache(max_tokens=tokens, n_slots=max_batch)
+        held = self._hold_batch_caches(max(sum(need[:max_batch]), PAGE_TOKENS), len(prompts), max_batch)
         return _generate(self.model, prompts, max_tokens, self._params(temperature, top_k, seed),
                          stop_ids=stop_ids, context=self.context, max_batch=min(max_batch, held.n_slots), cache=held)
+
+    def _hold_batch_caches(self, tokens: int, n_prompts: int, max_batch: int):
+        """One cache (with drafts: a pair) serves call after call, and with it the recorded graphs of its batch sizes; a call
+        that needs more room than any before gets a larger one."""
+        held = self._batch_cache
+        if held is None or held.n_pages * held.page_tokens < tokens or held.n_slots < min(max_batch, n_prompts):
+            self._batch_cache = self._draft_batch_cache = None
+            for model in (self.model, self.draft):
+                if model is not None:
+                    model.__dict__.pop("_decode_sessions", None)
+            held = self.model.new_cache(max_tokens=tokens, n_slots=max_batch)
+            if self.draft is not None:
+                self._draft_batch_cache = self.draft.new_cache(max_tokens=tokens, n_slots=max_batch)
+            self._batch_cache = held
+        return held
 
     def _need_model(self) -> None:
         if self.model is None:

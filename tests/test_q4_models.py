@@ -279,6 +279,44 @@ def test_drafted_samples_depend_on_seed_alone(model_dirs):
 
 
 @gpu
+def test_drafted_generation_keeps_its_caches_and_graphs(model_dirs, monkeypatch):
+    """Call after call on one pair of caches and the same recordings; a batch that thins out one by one moves to a smaller graph only where
+    it has halved; larger calls take the place of what was held, and nothing else keeps it."""
+    import gc
+    import weakref
+    from math_utils_b200.engine.decode_session import DecodeSession
+    recorded = []
+    record = DecodeSession._record_graph
+    monkeypatch.setattr(DecodeSession, "_record_graph", lambda self, *a: recorded.append(self.n) or record(self, *a))
+    llm = LLM(model_dirs["tiny_b"], Options(temperature=0.0, drafts=3, max_batch=16))            # 80 positions
+    thinning = [tokens_for(1031, 48 + 2 * i, i) for i in range(16)]
+    first = llm.generate(thinning, max_tokens=60, stop_ids=[])
+    assert [len(o) for o in first] == [32 - 2 * i for i in range(16)]
+    assert len(recorded) <= 5 and recorded[0] == 16 and all(b * 2 <= a for a, b in zip(recorded, recorded[1:]))
+    pair = llm._batch_cache, llm._draft_batch_cache
+    held, n = None, len(recorded)
+    for _ in range(4):
+        assert llm.generate(thinning, max_tokens=60, stop_ids=[]) == first
+        assert (llm._batch_cache, llm._draft_batch_cache) == pair and len(recorded) == n
+        gc.collect()
+        torch.cuda.synchronize()
+        now = torch.cuda.memory_allocated()
+        assert held is None or now - held <= 2 ** 20
+        held = now
+    for c in pair:
+        assert c.slots.n_free == 16 and c.free_pages(0) == c.n_pages
+    old = [weakref.ref(c) for c in pair]
+    del pair, c
+    llm.options = Options(temperature=0.0, drafts=3, max_batch=24)
+    assert len(llm.generate([thinning[0]] * 24, max_tokens=4, stop_ids=[])) == 24
+    gc.collect()
+    assert all(r() is None for r in old)
+    sessions = dict(llm.draft.__dict__["_decode_sessions"])
+    assert [len(o) for o in generate_drafted(llm.model, llm.draft, thinning[:2], 4, SamplingParams(0.0, 0, 0), 3, stop_ids=[])] == [4, 4]
+    assert dict(llm.draft.__dict__["_decode_sessions"]) == sessions
+
+
+@gpu
 def test_the_first_drafted_tokens_are_distributed_as_the_models(model_dirs):
     """The second token of 2,048 requests with one prompt, given the commonest first token: frequencies of the four likeliest
     against the model's own softmax, within 5 standard deviations of a binomial count."""
