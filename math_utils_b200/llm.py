@@ -70,7 +70,7 @@ class LLM:
             try:
                 self.draft = DecoderModel.from_dir(model_dir, dtype=o.dtype, device=self.device, weight_bits=4, row_bits=o.row_bits)
                 check_draftable(self.model, self.draft, self.model.new_cache(64, 1), self.draft.new_cache(64, 1))
-            except ValueError:
+            except Exception:              # whatever it was: a model without its draft would answer without drafts
                 self.unload()
                 raise
         self.current = model_dir

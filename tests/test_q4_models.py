@@ -225,6 +225,29 @@ def test_refused_combinations():
         LLM(options=Options(drafts=-1)).use("/nowhere")
 
 
+@pytest.mark.parametrize("error", [RuntimeError, MemoryError, ValueError])
+def test_a_draft_that_cannot_be_loaded_leaves_no_model(monkeypatch, error):
+    """Whatever ends the load of the draft, the model does not stay behind to answer without drafts."""
+    from math_utils_b200 import llm as module
+    loads = []
+
+    class Models:
+        @staticmethod
+        def from_dir(folder, **how):
+            loads.append(how["weight_bits"])
+            if len(loads) == 2:
+                raise error("no room")
+            return object()
+
+    monkeypatch.setattr(module, "DecoderModel", Models)
+    llm = LLM(options=Options(drafts=2))
+    with pytest.raises(error, match="no room"):
+        llm.use("/nowhere")
+    assert loads == [16, 4] and not llm.loaded and llm.draft is None
+    with pytest.raises(RuntimeError, match="no model loaded"):
+        llm.generate([[1, 2]])
+
+
 # ------------------------------------------------------------------------------------------------ drafted tokens
 def test_rooms_and_draws():
     class Model:
