@@ -68,7 +68,9 @@ class LLM:
         if o.drafts:
             from .engine.drafted import check_draftable
             try:
-                self.draft = DecoderModel.from_dir(model_dir, dtype=o.dtype, device=self.device, weight_bits=4, row_bits=o.row_bits)
+                # (a model in 4 bits is its own draft)
+                self.draft = self.model if o.weight_bits == 4 else DecoderModel.from_dir(
+                    model_dir, dtype=o.dtype, device=self.device, weight_bits=4, row_bits=o.row_bits)
                 check_draftable(self.model, self.draft, self.model.new_cache(64, 1), self.draft.new_cache(64, 1))
             except Exception:              # whatever it was: a model without its draft would answer without drafts
                 self.unload()

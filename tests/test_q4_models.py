@@ -248,6 +248,29 @@ def test_a_draft_that_cannot_be_loaded_leaves_no_model(monkeypatch, error):
         llm.generate([[1, 2]])
 
 
+def test_a_model_in_4_bits_is_its_own_draft(monkeypatch):
+    """Its draft would hold the same numbers: it is loaded once."""
+    from math_utils_b200 import llm as module
+    from math_utils_b200.engine import drafted
+    loads = []
+
+    class Models:
+        @staticmethod
+        def from_dir(folder, **how):
+            loads.append((how["weight_bits"], how["row_bits"]))
+            return Models()
+
+        def new_cache(self, *a):
+            return None
+
+    monkeypatch.setattr(module, "DecoderModel", Models)
+    monkeypatch.setattr(drafted, "check_draftable", lambda *a: None)
+    llm = LLM(options=Options(drafts=2, weight_bits=4, row_bits=8)).use("/nowhere")
+    assert loads == [(4, 8)] and llm.draft is llm.model
+    llm.use("/nowhere", Options(drafts=2))
+    assert loads[1:] == [(16, 16), (4, 16)] and llm.draft is not llm.model
+
+
 # ------------------------------------------------------------------------------------------------ drafted tokens
 def test_rooms_and_draws():
     class Model:
