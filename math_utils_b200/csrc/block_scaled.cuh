@@ -64,9 +64,11 @@ __device__ __forceinline__ uint2 e4m3_of_eight(const float (&v)[8], int b) {
 
 // Eight bfloat16 entries of a group as TWO codes each: hi = e4m3(v / 2^e), lo = e4m3((v - hi 2^e) / 2^(e - 4)), so that
 // v = hi 2^e + lo 2^(e - 4).  A bfloat16 has 8 significant bits, hi takes the upper 4 and leaves a remainder of at most
-// 2^-4 of v that is a multiple of 2^-7 of v's leading bit: 4 bits, which lo holds exactly.  (Entries below 2^-14 of the
-// group's largest lose what lies below 2^-22 of that largest one.)  The exponent byte of lo is b - 4; where b < 4 (a
-// group below 2^-115) its scale stays at 2^-127 and lo is made for that scale.
+// 2^-4 of v that is a multiple of 2^-7 of v's leading bit: 4 bits, which lo holds exactly while they are multiples of its least
+// step, 2^-13 2^e.  The group's largest entry lies above 224 2^e, so entries down to 2^-13 of it are held exactly and smaller ones
+// within 2^-14 2^e, which is less than 2^-21 of it.  Beside that entry's own product a float32 sum keeps no more; where its
+// weight is 0 the sum could, and does not here: a third piece would hold it, for half as much time again.  The exponent byte of lo is b - 4; where
+// b < 4 (a group below 2^-115) its scale stays at 2^-127 and lo is made for that scale.
 //
 // words: the entries as they lie in memory, two a word.
 __device__ __forceinline__ int low_exponent(int b) { return b > 4 ? b - 4 : 0; }

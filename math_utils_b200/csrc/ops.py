@@ -1863,9 +1863,9 @@ Q4_NORM_WIDTH = 8192           # the widest LayerNorm that a product makes of it
 def linear_q4(x, weight: Q4Weight, bias: Optional[torch.Tensor] = None, act: Optional[str] = None,
               residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
               out_dtype: Optional[torch.dtype] = None, way: int = 0) -> torch.Tensor:
-    """act(x @ W^T + bias) + residual with W in 4 bits.  ``x``: bfloat16 [m, k] with unit stride along k (taken as they
-    are: cut into two 8-bit pieces that together hold them), ``Q8Rows``, or a ``NormedInput`` (of up to 8 rows the norm
-    is made inside the kernel).  Sums are float32;
+    """act(x @ W^T + bias) + residual with W in 4 bits.  ``x``: bfloat16 [m, k] with unit stride along k (cut into two 8-bit
+    pieces: an entry is held exactly down to 2^-13 of the largest of its 32 neighbours, a smaller one within 2^-21 of that
+    largest), ``Q8Rows``, or a ``NormedInput`` (of up to 8 rows the norm is made inside the kernel).  Sums are float32;
     ``out`` bfloat16 (the default) or float32; ``bias`` float32 [n], ``residual`` float32 [m, n], which may be ``out``.
     A row that holds an infinity or NaN gives NaN.  ``way``: 0, or which kernel runs: 1 + b the one for few rows (up to
     64) with b blocks a tile (0: the library chooses), -64, -128, -192 or -256 the one for many with tiles that

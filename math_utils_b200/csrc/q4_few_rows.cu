@@ -10,7 +10,7 @@
 //   * K is cut over the blocks of a cluster (any number up to 8) so that tiles x splits fill the SMs; the partial tiles
 //     meet in distributed shared memory and are added in rank order.  They lie on the stages, which nothing reads once
 //     every block of the cluster has its accumulator;
-//   * bfloat16 rows are two pieces, each e4m3, that together hold them exactly: they lie one behind the other,
+//   * bfloat16 rows are two pieces, each e4m3, that together hold them (block_scaled.cuh says how exactly): they lie one behind the other,
 //     one instruction multiplies both (up to 32 columns take the instruction 40 cycles, however few they are), and their
 //     accumulators are added where they are read.  Up to 8 rows are cut here, by eight warps, two a stage (every block cuts its own share of k: 1.2 us a
 //     launch at 8 rows, 3.5 at 16, where a launch before costs 1.4); more rows come cut by a launch of their own

@@ -3,7 +3,7 @@
 //
 // The instruction multiplies e4m3 by e2m1 at the 8-bit rate, 128 x 192 x 32 in 96 cycles, and applies both exponents, so the
 // weights are never expanded: TMA spreads the packed codes in shared memory, 12 KB of L2 for 192 columns of 128 of k.
-// bfloat16 rows come as two 8-bit pieces that together hold them exactly (q8_rows.cu): two products a step into one
+// bfloat16 rows come as two 8-bit pieces that together hold them (block_scaled.cuh says how exactly): two products a step into one
 // accumulator, the rate of a bfloat16 product.
 //
 // Persistent: a block an SM walks over the tiles; the ring of stages runs on across tiles, two accumulators in tensor memory

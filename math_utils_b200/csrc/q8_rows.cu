@@ -2,7 +2,7 @@
 //
 // mu_quantize_q4          a weight matrix to e2m1 codes and exponent bytes.
 // mu_quantize_q8          rows to e4m3 codes and exponent bytes; with two pieces, bfloat16 rows to codes that together hold
-//                         them exactly.
+//                         them (block_scaled.cuh says how exactly).
 // mu_residual_add_norm_q8 x += (mult * y + mult2 * y2) * scale on the float32 stream, then h = x / sqrt(mean(x^2) + eps) *
 //                         weight, written in 8 bits.
 //
@@ -298,7 +298,9 @@ int launch_quantize_q8(const void* x, long long ldx, int is_bf16, int m, int k, 
     // a block's threads along a row and its rows: whole warps of a row where it has as many eights
     const int along = eights >= 256 ? 256 : eights >= 128 ? 128 : eights >= 64 ? 64 : eights >= 32 ? 32 : 16;
     const int deep = 256 / along;
-    const bool many = rows * (long long)eights >= 2ll * 148 * 2048;
+    const int sms = sm_count();
+    if (sms <= 0) return MU_ERR_LAUNCH;
+    const bool many = rows * (long long)eights >= 2ll * sms * 2048;
     const int each = many ? 4 : 1;
     const dim3 block(along, deep), grid((unsigned)((rows + deep * each - 1) / (deep * each)), (eights + along - 1) / along);
     if (grid.y > 65535) return MU_ERR_UNSUPPORTED_SIZE;

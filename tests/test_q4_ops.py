@@ -253,6 +253,25 @@ def test_products_give_the_same_bits_again_and_for_a_row_among_others():
 
 
 @gpu
+@pytest.mark.parametrize("m", [3, 8, 20, 64, 200])
+def test_what_the_two_pieces_of_a_row_hold(m):
+    """Weights of a unit matrix give each entry by itself, the group's largest among those that meet only zeros: entries down to 2^-13
+    of it come back as they are, smaller ones within half the second piece's least step, 2^-14 of the scale, which the largest
+    entry is more than 224 of."""
+    k = 256
+    gen = torch.Generator().manual_seed(m)
+    x = (1.0 + torch.rand((m, k), generator=gen)) * torch.exp2(-torch.randint(0, 30, (m, k), generator=gen).float())
+    x = (x * torch.where(torch.rand((m, k), generator=gen) < 0.5, -1.0, 1.0)).bfloat16()
+    x[:, ::32] = ((1.0 + torch.rand((m, k // 32), generator=gen)) * 8.0).bfloat16()
+    got = f64(ops.linear_q4(x.cuda(), ops.quantize_q4(torch.eye(k).cuda()), out_dtype=torch.float32)).reshape(m, -1, 32)
+    want = f64(x).reshape(m, -1, 32)
+    top = np.abs(want).max(axis=2, keepdims=True)
+    exact = np.abs(want) >= 2.0 ** -13 * top
+    assert exact.any() and not exact.all() and np.array_equal(got[exact], want[exact])
+    assert (np.abs(got - want) <= 2.0 ** -14 / 224 * top).all() and 2.0 ** -14 / 224 < 2.0 ** -21
+
+
+@gpu
 def test_a_row_that_is_no_number_leaves_the_others():
     x = normal((5, 256), 1).bfloat16()
     x[1, 7], x[3, 200] = float("inf"), float("nan")
