@@ -2059,7 +2059,8 @@ def verify_drafts(logits: torch.Tensor, draft_logits: Optional[torch.Tensor], dr
     draws[i] * q(draft i) < p(draft i).  The token behind the taken ones comes from max(p - q, 0) where a draft was not
     taken and from p where none is left: the first index at which the running sum passes draws[drafts] of the whole.
     ``tokens``: the drafts taken, that token, then -1; ``kept`` how many drafts were taken.  Greedy: a draft is taken
-    while it is its row's first maximum, which is also the token that follows."""
+    while it is its row's first maximum, which is also the token that follows.  All decisions are those of the formulas in 64
+    bits; a row without a finite logit or with a NaN takes no draft and gives its first maximum, a NaN above every number."""
     if logits.dtype != torch.float32 or logits.dim() != 3 or logits.stride(2) != 1 or logits.shape[1] < 1 or logits.shape[2] < 1:
         raise KernelError("verify_drafts: logits are float32 [batch, drafts + 1, vocab] with unit inner stride")
     b, g, vocab = logits.shape[0], logits.shape[1] - 1, logits.shape[2]

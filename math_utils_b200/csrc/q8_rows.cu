@@ -6,9 +6,10 @@
 // mu_residual_add_norm_q8 x += (mult * y + mult2 * y2) * scale on the float32 stream, then h = x / sqrt(mean(x^2) + eps) *
 //                         weight, written in 8 bits.
 //
-// What bounds them is bytes: the norm reads 8 and writes 4 + 1 + 1/32 for an entry: 4,096 x 8,192 in 81-85 us, 5.1-5.4 TB/s, four
-// fifths of what a copy reaches (two turns a thread in blocks of 512 took 87: fewer blocks to fill one another's gaps); 8 x 2,048 in 2.7.
-// The two pieces of 2,048 x 1,024 rows 2.5 us before a product, of 2,048 x 2,048 some 4.
+// What bounds them is bytes: the norm reads 8 and writes 4 + 1 + 1/32 for an entry: 4,096 x 8,192 in 82-87 us, 5.0-5.3 TB/s, four
+// fifths of what a copy reaches (two turns a thread in blocks of 512 took 87: fewer blocks to fill one another's gaps); 8 x 2,048 in 2.6.
+// The two pieces of 2,048 x 1,024 rows 4 us before a product.  A weight of 6,400 x 1,600 to 4 bits, once at load: 25 us; of 16,384 x 8,192:
+// 253 (a thread reads its 32 entries one by one).
 #include "addend.cuh"
 #include "block_scaled.cuh"
 

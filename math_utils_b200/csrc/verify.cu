@@ -14,10 +14,10 @@
 // by the reading.  With one: the k largest logits, as a list (verify_top_kernel).  Greedy: the first maximum.  The second
 // decides, a block or a cluster of blocks a sequence, and draws the token: from the lists (verify_list_kernel), or by a
 // walk over the one row pair that matters, each block of the cluster its share of the vocabulary (verify_walk_kernel).
-// What bounds them, on a B200: the first launch reads 704 rows of 50,257 logits (141 MB) in 35 us, 4.1 TB/s, a wave and two thirds
-// of blocks behind the first; the walk for 64 sequences takes another 36, two waves of clusters of some 11 us (masses 4, rows 2, three
-// cluster barriers and the decision the rest).  With a top_k of 40, 8 sequences of 4 drafts: 17.4 us for both, of
-// which the first reads 1.5, finds the floor 1.2, gathers 1.7, ranks 1, joins 2.6.
+// What bounds them, on a B200: the first launch reads 704 rows of 50,257 logits (141 MB) in 27 us, 5.3 TB/s, one such launch after another;
+// the walk behind it for 64 sequences takes another 47, two waves of clusters: some 33 clusters of eight go at a time (rows that are still
+// in the L2, no drafts: 8 to 32 sequences 13 to 17 us, 36 to 64 21 to 25).  With a top_k of 40, 8 sequences of 4 drafts:
+// 17.3 us for both, 11.9 the first, which reads 1.5, finds the floor 1.2, gathers 1.7, ranks 1, joins 2.6.
 // The walk is in 64 bits, exponentials included: with 50,000 tokens in a row a running sum that is off by 1e-7 of the whole
 // would give another token once in a hundred draws.  The exponentials are made by a table
 // (exp_of).  Decisions about drafts are the 64-bit formula's too: the first launch's 32-bit sums decide where their error cannot matter, and
