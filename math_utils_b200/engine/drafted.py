@@ -46,6 +46,16 @@ def room_for_drafts(model, draft, lengths: Sequence[int], drafts: int, context: 
     return max(0, min([drafts] + [most - n - 1 for n in lengths]))
 
 
+def acquire_pair(cache, draft_cache):
+    """A slot of each cache, or of neither."""
+    slot = cache.acquire()
+    try:
+        return slot, draft_cache.acquire()
+    except Exception:
+        cache.release(slot)
+        raise
+
+
 def run_drafted(model, draft, cache, draft_cache, params: SamplingParams, states, stop_ids, max_tokens: int, context: int,
                 drafts: int, kept_slots: Optional[Sequence] = None, first_sample: Optional[list] = None,
                 counts: Optional[dict] = None) -> None:
@@ -65,7 +75,7 @@ def run_drafted(model, draft, cache, draft_cache, params: SamplingParams, states
             if max_tokens <= 0 or st.held + len(st.prompt) >= context:
                 st.finished, st.reason = True, "max_tokens" if max_tokens <= 0 else "context"
                 continue
-            slots[k] = kept_slots[k] if kept_slots is not None else (cache.acquire(), draft_cache.acquire())
+            slots[k] = kept_slots[k] if kept_slots is not None else acquire_pair(cache, draft_cache)
             live.append(k)
         if not live:
             return

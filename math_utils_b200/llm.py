@@ -127,11 +127,13 @@ class LLM:
         if len(ids) + 8 >= limit:
             raise ValueError("the prompt alone does not fit in the context")
         if self._slot is None:
-            self._slot = self._cache.acquire()
-            if self.draft is not None:
+            if self.draft is None:
+                self._slot = self._cache.acquire()
+            else:
+                from .engine.drafted import acquire_pair
                 if self._draft_cache is None:
                     self._draft_cache = self.draft.new_cache(max_tokens=-(-limit // 64) * 64, n_slots=1)
-                self._draft_slot = self._draft_cache.acquire()
+                self._slot, self._draft_slot = acquire_pair(self._cache, self._draft_cache)
         # the conversation so far counts toward the context rule; the turn keys the sampling stream
         state = RequestState(self._turns, list(ids), held=held)
         self._turns += 1

@@ -226,3 +226,34 @@ def test_a_conversation_up_to_the_end_of_the_context(monkeypatch):
             said += ids + want
             for model, cache, slot in zip((world.model, world.draft), world.caches, pair):
                 assert cache.length(slot) == len(said) and model.memory.read(slot, len(said)) == said
+
+
+def test_slots_are_had_in_pairs(monkeypatch):
+    """Where the draft's cache has no slot left, or cannot be made, none of the model's stays taken."""
+    from math_utils_b200 import LLM, Options
+    from math_utils_b200.cache import CacheFull
+    world = World(monkeypatch, [5, 5], 3, 100, 2)
+    taken = world.caches[1].acquire()
+    with pytest.raises(CacheFull):
+        world.run([[1, 2, 3], [4, 5]], (), 3, 100, 2)
+    assert world.caches[0].slots.n_free == 2 and world.caches[1].slots.n_free == 1
+    world.caches[1].release(taken)
+    assert [len(s.produced) for s in world.run([[1, 2, 3], [4, 5]], (), 3, 100, 2)[0]] == [3, 3]
+
+    class Model:
+        max_positions = 100
+
+        def __init__(self, cache):
+            self.cache = cache
+
+        def new_cache(self, **how):
+            if self.cache is None:
+                raise MemoryError("no room")
+            return self.cache
+
+    llm = LLM(options=Options(drafts=2))
+    llm.model, llm.draft = Model(world.caches[0]), Model(None)
+    for _ in range(2):
+        with pytest.raises(MemoryError):
+            llm.prompt([1, 2, 3])
+        assert llm._slot is None and world.caches[0].slots.n_free == 2
